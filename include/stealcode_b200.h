@@ -444,6 +444,122 @@ int sc_rnnt_state(const sc_rnnt_decoder *r, int64_t stream_idx, float *h,
                   float *c, int32_t *last_token);
 int sc_rnnt_destroy(sc_rnnt_decoder *r);
 
+/* ---- paged 8-bit key/value cache ---------------------------------------------
+ * Attention over a long past beside the encoder's short rings: keys and
+ * values held in 8 bits with one f32 scale per `block` tokens and kv head,
+ * in pages of `page` tokens that several sequences can share.  No
+ * counterpart in the reference.
+ *
+ * The caller owns all memory (device):
+ *   k, v             int8 [n_layers][n_pages][n_kv_heads][page][head_dim]
+ *   k_scale, v_scale f32  [n_layers][n_pages][n_kv_heads][page / block]
+ *   table   int32 [n_seqs][max_pages]  page ids of each sequence's tokens in
+ *           order; -1 = none (entries past ceil(length / page) are -1)
+ *   length  int32 [n_seqs]  tokens of each sequence
+ *   refs    int32 [n_pages] table entries that name a page; 0 = free
+ *   status  uint32 [1]      sticky SC_KV8_* bits, 0 at first
+ * A new cache has table -1 and length, refs, status 0; codes and scales need
+ * no initialisation.  head_dim is 64 or 128; block 16, 32 or 64; page a
+ * multiple of block, at most 1024; k and v 16-byte aligned.
+ *
+ * A step of some sequences: sc_kv8_reserve (pages for the new tokens; the
+ * lengths grow), then per layer sc_kv8_append (their keys and values) and
+ * sc_kv8_attend (their queries).  append, attend and rows work on the LAST
+ * tokens of each sequence.  All calls are asynchronous on stream; calls on
+ * one cache have to be ordered by the caller.
+ *
+ * Failures that only the device can see set bits of the status word.  A
+ * reserve, fork or compact that fails changes nothing; while a bit is set,
+ * reserve, fork, compact and append do nothing (release and slide run), until
+ * the caller writes 0. */
+#define SC_KV8_POOL_FULL 1u     /* too few free pages */
+#define SC_KV8_TABLE_FULL 2u    /* a sequence past max_pages */
+#define SC_KV8_BAD_SEQUENCE 4u  /* sequence id outside the cache or named twice, or a negative count */
+#define SC_KV8_BAD_PAGE 8u      /* page id outside the cache, or an append without a reserved page */
+#define SC_KV8_WAIT_TIMEOUT 16u /* a bounded device-side wait gave up */
+
+#define SC_DTYPE_F32 0
+#define SC_DTYPE_F16 1
+#define SC_DTYPE_BF16 2
+
+typedef struct {
+  int8_t *k, *v;
+  float *k_scale, *v_scale;
+  int32_t *table, *length, *refs;
+  uint32_t *status;
+  int64_t n_layers, n_pages, n_seqs, max_pages;
+  int32_t n_kv_heads, head_dim, page, block;
+} sc_kv8_cache;
+
+/* The rows of a call: m sequences, row r of the i-th (sequence seqs[i], or i
+ * when seqs is NULL) at packed row cu[i] + r, cu[i + 1] - cu[i] rows of it
+ * (cu NULL: n rows each), at most n; `total` packed rows in all.  seqs, cu:
+ * device arrays.  No sequence is named twice. */
+typedef struct {
+  const int32_t *seqs, *cu;
+  int64_t m, n, total;
+} sc_kv8_batch;
+
+/* Quantise new rows k, v into the sequences' last tokens of one layer.
+ * Element (row, head, d) of k is k[row * k_row + head * k_head + d].  A
+ * block's scale is max |x| * (1 / 127) over its rows (finite elements); it grows
+ * when later rows of the block are larger, and the older codes are rounded
+ * to the new scale.  NaN is stored as 0, Inf as the block's largest value. */
+int sc_kv8_append(const sc_kv8_cache *c, int64_t layer,
+                  const sc_kv8_batch *b, const void *k, int64_t k_row,
+                  int64_t k_head, const void *v, int64_t v_row,
+                  int64_t v_head, int32_t dtype, void *stream);
+/* The stored values of the sequences' last tokens, code * scale: k, v
+ * [total][n_kv_heads][head_dim] of dtype (either may be NULL; 16-byte
+ * aligned).  Tokens without a page read as 0. */
+int sc_kv8_rows(const sc_kv8_cache *c, int64_t layer, const sc_kv8_batch *b,
+                void *k, void *v, int32_t dtype, void *stream);
+
+/* Attention of the sequences' last tokens (their rows of q) over the
+ * sequences: query head h reads kv head h / (n_heads / n_kv_heads); a query
+ * at position p sees the tokens t <= p that still have a page and, with
+ * window > 0, t > p - window or t < sinks.  out = softmax(scale * q k) v in
+ * q's dtype, lse (f32 [total][n_heads], may be NULL) the log of the sum of
+ * exponentials; a query that sees nothing gets 0 and -inf.  max_len: no
+ * sequence is longer (<= 0: unknown); a hint that sizes the launch.
+ * workspace: sc_kv8_attend_workspace_bytes (of the current device), 256-byte
+ * aligned, zeroed once before its first use; calls that may overlap need one
+ * each. */
+int64_t sc_kv8_attend_workspace_bytes(void);
+int sc_kv8_attend(const sc_kv8_cache *c, int64_t layer,
+                  const sc_kv8_batch *b, const void *q, int64_t q_row,
+                  int64_t q_head, int32_t n_heads, float scale,
+                  int64_t window, int64_t sinks, int64_t max_len, void *out,
+                  int64_t out_row, int64_t out_head, float *lse,
+                  int32_t dtype, void *workspace, int64_t workspace_bytes,
+                  void *stream);
+
+/* Page bookkeeping, on the device and without a copy to the host.  Free pages
+ * are taken lowest id first, in the order of the call's sequences.  seqs NULL
+ * means sequences 0 .. m - 1; m <= n_seqs.  workspace:
+ * sc_kv8_page_workspace_bytes, 256-byte aligned.
+ * reserve: counts[i] more tokens for sequence seqs[i]; its length grows.
+ * fork: children[i] becomes a copy of parents[i] (all pairs at once, so
+ *   parents may be children too): full pages are shared, a partly filled
+ *   last page is copied, what the child held before is released.
+ * release: the sequences' pages go back, their lengths become 0.
+ * slide: the pages that no query at or after the last token can see under
+ *   this window and these sinks go back; lengths stay.
+ * compact: the pages in use move to the lowest ids. */
+int64_t sc_kv8_page_workspace_bytes(const sc_kv8_cache *c);
+int sc_kv8_reserve(const sc_kv8_cache *c, const int32_t *seqs,
+                   const int32_t *counts, int64_t m, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+int sc_kv8_fork(const sc_kv8_cache *c, const int32_t *parents,
+                const int32_t *children, int64_t m, void *workspace,
+                int64_t workspace_bytes, void *stream);
+int sc_kv8_release(const sc_kv8_cache *c, const int32_t *seqs, int64_t m,
+                   void *stream);
+int sc_kv8_slide(const sc_kv8_cache *c, const int32_t *seqs, int64_t m,
+                 int64_t window, int64_t sinks, void *stream);
+int sc_kv8_compact(const sc_kv8_cache *c, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -105,6 +105,17 @@ SIGNATURES = {
     "sc_attn_stream_ring": (c_int, [_P, _I, _P, _P, _I, _P, _P, _I, _I, _P, _I,
                                     _P, _P, _I, _I, _I, c_float, _I, _I, _I,
                                     _I, _I, _I, _P, _I, _P]),
+    "sc_kv8_append": (c_int, [_P, _I, _P, _P, _I, _I, _P, _I, _I, c_int32, _P]),
+    "sc_kv8_rows": (c_int, [_P, _I, _P, _P, _P, c_int32, _P]),
+    "sc_kv8_attend_workspace_bytes": (c_int64, []),
+    "sc_kv8_attend": (c_int, [_P, _I, _P, _P, _I, _I, c_int32, c_float, _I, _I, _I, _P, _I, _I, _P, c_int32, _P, _I,
+                              _P]),
+    "sc_kv8_page_workspace_bytes": (c_int64, [_P]),
+    "sc_kv8_reserve": (c_int, [_P, _P, _P, _I, _P, _I, _P]),
+    "sc_kv8_fork": (c_int, [_P, _P, _P, _I, _P, _I, _P]),
+    "sc_kv8_release": (c_int, [_P, _P, _I, _P]),
+    "sc_kv8_slide": (c_int, [_P, _P, _I, _I, _I, _P]),
+    "sc_kv8_compact": (c_int, [_P, _P, _I, _P]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():

@@ -1,0 +1,190 @@
+// kv8_work.cuh -- how an attention call's work is shared out over the blocks
+// of a launch.
+//
+// For one (sequence, kv head) the query rows are the pairs (token, query
+// head of that kv head), token-major; an item is ROWS of them, and its keys
+// are the tiles of TILE consecutive tokens that hold a token some row sees:
+// tiles [0, a) of the first `sinks` tokens, then tiles [b, c) of the window.
+// All items' tiles, one after the other, are cut into equal contiguous
+// shares, one per block, whatever the sequences' lengths: a block computes
+// whole items and at most two parts of items (the end of one, the start of
+// another).  Parts go to the workspace; the block that finishes an item last
+// joins its parts in order, so the result does not depend on who was last.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace sc {
+namespace kv8 {
+
+struct WorkGrid {
+  int group;       // query heads per kv head
+  int per_seq;     // items per sequence and kv head, at most
+  int entries;     // m * per_seq
+  int min_share;   // tiles; fewer blocks work when there are few tiles
+  int32_t *count;  // [blocks] parts done of the item that starts in a block
+  float *parts;    // [2 * blocks] parts
+};
+
+struct Entry {
+  int i, s;         // entry of the batch, sequence (-1: none)
+  int64_t row0;     // first packed token
+  int first;        // position of that token
+  int r0, r1;       // rows [r0, r1) of the sequence
+  int p_lo, p_hi;   // positions of the first and the last row
+  int a, b, c;
+  __device__ __forceinline__ int tiles() const { return a + c - b; }
+  __device__ __forceinline__ int cost() const { return max(1, tiles()); }
+  __device__ __forceinline__ int tile(int x) const { return x < a ? x : b + x - a; }
+};
+
+// False when entry e has no rows.
+template <int ROWS, int TILE>
+__device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g, int e, Entry &o) {
+  o.i = e / g.per_seq;
+  int count;
+  p.b.rows(o.i, o.row0, count);
+  o.r0 = (e - o.i * g.per_seq) * ROWS;
+  const int rows = count * g.group;
+  if (o.r0 >= rows) return false;
+  o.r1 = min(rows, o.r0 + ROWS);
+  o.s = p.b.seq(o.i, p.c.n_seqs);
+  const int len = o.s < 0 ? 0 : seq_length(p.c, o.s);
+  o.first = len - count;
+  o.p_lo = o.first + o.r0 / g.group;
+  o.p_hi = o.first + (o.r1 - 1) / g.group;
+  o.a = o.b = o.c = 0;
+  if (o.p_hi >= 0) {
+    o.c = o.p_hi / TILE + 1;
+    if (p.window > 0) {
+      o.b = max(0, max(o.p_lo, 0) - p.window + 1) / TILE;
+      o.a = min((min(p.sinks, o.p_hi + 1) + TILE - 1) / TILE, o.b);
+    }
+  }
+  return true;
+}
+
+// A block's share [pos, end) of all tiles and the entry that holds pos.
+struct Share {
+  int64_t pos, end, total;
+  int blocks;       // blocks that have a share
+  int e;            // entry
+  int64_t at;       // first tile of entry e
+};
+
+// First block of `blocks` whose share reaches past tile `pos`.
+__device__ __forceinline__ int block_of(int64_t pos, int64_t total, int blocks) {
+  return (int)(((pos + 1) * blocks - 1) / total);
+}
+
+struct ShareScratch {
+  int64_t warp[32];
+  int e;
+  int64_t at;
+};
+
+// All threads of the block call; false when the block has nothing to do.
+template <int ROWS, int TILE, int THREADS>
+__device__ bool find_share(const AttendArgs &p, const WorkGrid &g, ShareScratch &sh, Share &o) {
+  const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (g.entries + THREADS - 1) / THREADS;
+  const int e0 = min(tid * per, g.entries), e1 = min(e0 + per, g.entries);
+  int64_t mine = 0;
+  Entry en;
+  for (int e = e0; e < e1; e++)
+    if (get_entry<ROWS, TILE>(p, g, e, en)) mine += (int64_t)en.cost() * p.c.kv;
+  int64_t x = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  if (lane == 31) sh.warp[warp] = x;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; w++) {
+    if (w < warp) before += sh.warp[w];
+    total += sh.warp[w];
+  }
+  const int64_t start = before + x - mine;
+  o.total = total;
+  const int64_t most = (total + g.min_share - 1) / g.min_share;
+  o.blocks = (int)(most < (int64_t)gridDim.x ? most : (int64_t)gridDim.x);
+  if ((int)blockIdx.x >= o.blocks) return false;
+  o.pos = (int64_t)blockIdx.x * total / o.blocks;
+  o.end = ((int64_t)blockIdx.x + 1) * total / o.blocks;
+  if (o.pos >= start && o.pos < start + mine) {
+    int64_t at = start;
+    for (int e = e0; e < e1; e++) {
+      if (!get_entry<ROWS, TILE>(p, g, e, en)) continue;
+      const int64_t n = (int64_t)en.cost() * p.c.kv;
+      if (o.pos < at + n) {
+        sh.e = e;
+        sh.at = at;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  o.e = sh.e;
+  o.at = sh.at;
+  return o.pos < o.end;
+}
+
+// One piece of the share: tiles [t0, t1) of an item.
+struct Piece {
+  int head;
+  int t0, t1;
+  bool whole, starts;  // the whole item; the piece holds the item's first tile
+  int c0, parts;       // block in which the item starts, and its parts
+};
+
+// Moves to the share's next piece (entry in `en`); false at its end.
+template <int ROWS, int TILE>
+__device__ __forceinline__ bool next_piece(const AttendArgs &p, const WorkGrid &g, Share &o, Entry &en, Piece &q) {
+  if (o.pos >= o.end) return false;
+  while (true) {
+    if (!get_entry<ROWS, TILE>(p, g, o.e, en)) {
+      o.e = (en.i + 1) * g.per_seq;  // the sequence has no more rows
+      continue;
+    }
+    const int64_t n = (int64_t)en.cost() * p.c.kv;
+    if (o.pos < o.at + n) break;
+    o.at += n;
+    o.e++;
+  }
+  const int cost = en.cost();
+  const int64_t off = o.pos - o.at;
+  q.head = (int)(off / cost);
+  q.t0 = (int)(off - (int64_t)q.head * cost);
+  q.t1 = (int)min((int64_t)cost, q.t0 + (o.end - o.pos));
+  const int64_t s0 = o.pos - q.t0;
+  o.pos += q.t1 - q.t0;
+  q.starts = q.t0 == 0;
+  q.whole = q.starts && q.t1 == cost;
+  q.c0 = q.starts ? (int)blockIdx.x : block_of(s0, o.total, o.blocks);
+  q.parts = q.t1 == cost ? (int)blockIdx.x - q.c0 + 1 : block_of(s0 + cost - 1, o.total, o.blocks) - q.c0 + 1;
+  return true;
+}
+
+// Workspace slot of part k of the item that starts in block c0.
+__device__ __forceinline__ int part_slot(int c0, int k) { return k == 0 ? 2 * c0 + 1 : 2 * (c0 + k); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kMaxBlocks = 4096;  // counters at the start of the workspace
+
+}  // namespace kv8
+}  // namespace sc
