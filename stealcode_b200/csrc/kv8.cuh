@@ -135,6 +135,9 @@ struct AttendArgs {
 // to be zero before the first call and is zero again after each call.
 size_t attend_ws_bytes(int sm_count);
 int attend(const AttendArgs &a, int sm_count, cudaStream_t st);
+// kv8_attend_tile.cu: the same for many rows per kv head
+size_t tile_ws_bytes(int sm_count);
+int attend_tile(const AttendArgs &a, int sm_count, cudaStream_t st);
 
 struct PageArgs {
   int8_t *k, *v;

@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
 
 size_t attend_ws_bytes(int sm_count) {
   const size_t step = (size_t)sm_count * 4 * 2 * 16 * 130 * 4;
-  return kMaxBlocks * 4 + step;
+  const size_t tile = tile_ws_bytes(sm_count);
+  return kMaxBlocks * 4 + (step > tile ? step : tile);
 }
 
 template <int D, int NT, typename T>
@@ -472,6 +473,7 @@ static int step(const AttendArgs &a, int sm_count, cudaStream_t st) {
 
 int attend(const AttendArgs &a, int sm_count, cudaStream_t st) {
   if (a.b.m == 0 || a.b.n == 0 || a.b.total == 0) return kOk;
+  if ((int64_t)a.b.n * (a.n_heads / a.c.kv) > 32) return attend_tile(a, sm_count, st);
   if (a.dtype == SC_DTYPE_F32) return step<float>(a, sm_count, st);
   if (a.dtype == SC_DTYPE_F16) return step<__half>(a, sm_count, st);
   return step<__nv_bfloat16>(a, sm_count, st);

@@ -1,0 +1,682 @@
+// kv8_attend_tile.cu -- attention over the paged 8-bit cache for many query
+// rows per kv head (prompts, long chunks), on the tensor cores' own memory.
+// Formulas and numerics are kv8_attend.cu's; the parts of split items and the
+// sharing-out are kv8_work.cuh's.
+//
+// A block takes 256 rows (token, query head of the group) as two tiles of 128
+// and walks the keys 128 at a time:
+//   warps 0-3, 4-7  softmax of row tile 0, 1: a thread holds one row, reads
+//                   its 128 scores from tensor memory, writes the weights
+//                   back over them as f16, and rescales the output
+//                   accumulator when its maximum has grown by more than 2^7;
+//   warps 8-11      read the codes of K and V (16-byte loads, one tile ahead
+//                   in registers) and write them to shared memory as f16
+//                   operands: K as it lies (its depth is contiguous), V
+//                   transposed by stmatrix;
+//   warp 12         issues S = Q K^T and O += W V; while one row tile is in
+//                   its softmax the other's products run.
+// The codes pass through the converters once for 256 rows, so their cost is
+// shared by all query heads of the group.
+//
+// Operands are no-swizzle K-major: element (row, k) of an operand of R rows
+// is at ((k / 8) * R + row) * 16 + (k % 8) * 2 bytes.  Within 64 elements of
+// V's depth the order is n = 8 p + 2 t + e for element 16 t + 2 p + e: what a
+// lane's 16 loaded bytes give stmatrix without a shuffle; the epilogue undoes
+// it.  f32 queries and weights are hi + lo pairs of f16: twice the products.
+#include <atomic>
+
+#include "kv8_work.cuh"
+#include "sc_kernels.cuh"
+#include "sc_tcgen05.cuh"
+
+namespace sc {
+namespace kv8 {
+
+constexpr int kTileRows = 256, kTileKeys = 128;
+constexpr int kTileThreads = 512;  // 13 warps work; setmaxnreg needs whole warpgroups
+constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
+constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
+
+template <int D, bool SPLIT>
+struct TileCfg {
+  static constexpr int kStages = SPLIT && D == 128 ? 1 : 2;
+  static constexpr int kQ = 128 * D * 2;   // bytes of one row tile's queries (one term)
+  static constexpr int kKv = 128 * D * 2;  // bytes of one K or V tile
+  static constexpr int kTerms = SPLIT ? 2 : 1;
+  static constexpr int kOperands = 2 * kTerms * kQ + 2 * kStages * kKv;
+};
+
+struct TileShared {  // after the operands
+  uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  // a key tile's 16-token groups: score factor ks, log2(vs), weight factor
+  // vs * 2^8, and whether the group has a page; four tiles deep, so a slot is
+  // written again only after both softmaxes have read it
+  float kf[4][8], lv[4][8], wf[4][8];
+  uint32_t live[4][4];  // two bits from each converter warp
+  ShareScratch share;
+  uint32_t tmem;
+  int last;
+};
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Bytes (0, 1) or (2, 3) of a word of codes + 128, as two f16 (0x6400 | u is
+// 1024 + u).
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
+  const uint32_t u = __byte_perm(w, 0x64646464u, sel);
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void stmatrix_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
+}
+
+// A row of q as f16 (hi and, for f32, lo), scaled by a power of two with the
+// sign of the score factor; returns the factor of its scores.
+template <int D, typename T>
+__device__ __forceinline__ float load_query(const T *src, bool vec, float scale, unsigned char *hi, unsigned char *lo) {
+  constexpr int N = 16 / sizeof(T);  // elements of a 16-byte load
+  float top = 0.0f;
+  if (vec) {
+#pragma unroll 8
+    for (int i = 0; i < D / N; i++) {
+      const uint4 w = __ldg((const uint4 *)src + i);
+      const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+      for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+    }
+  } else {
+#pragma unroll 8
+    for (int i = 0; i < D; i++) top = fmaxf(top, fabsf(to_f32<T>(src[i])));
+  }
+  int k = 0;
+  if (top > 0.0f) k = min(100, 140 - (int)(__float_as_uint(top) >> 23));
+  float up = __uint_as_float((uint32_t)(127 + k) << 23);
+  const float down = __uint_as_float((uint32_t)(127 - k) << 23);
+  // score factors stay positive: a group's largest score is its largest product
+  if (scale < 0.0f) up = -up;
+  if (scale == 0.0f) up = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < D / 8; i++) {
+    float x[8];
+    if (vec) {
+#pragma unroll
+      for (int j = 0; j < 8 / N; j++) {
+        const uint4 w = __ldg((const uint4 *)src + i * (8 / N) + j);
+        const T *y = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int e = 0; e < N; e++) x[j * N + e] = to_f32<T>(y[e]) * up;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = to_f32<T>(src[i * 8 + e]) * up;
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      h[e] = pack_h2(x[2 * e], x[2 * e + 1]);
+      if (sizeof(T) == 4) {
+        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
+        l[e] = pack_h2(x[2 * e] - b.x, x[2 * e + 1] - b.y);
+      }
+    }
+    *(uint4 *)(hi + i * 2048) = make_uint4(h[0], h[1], h[2], h[3]);
+    if (sizeof(T) == 4) *(uint4 *)(lo + i * 2048) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+  return fabsf(scale) * kLog2e * down;
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attend_tile_kernel(const __grid_constant__ AttendArgs p, const __grid_constant__ WorkGrid g, int vec_q, int vec_o) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  using C = TileCfg<D, SPLIT>;
+  constexpr int NS = C::kStages;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *qs = smem;                             // [2 row tiles][terms] queries
+  unsigned char *kt = smem + 2 * C::kTerms * C::kQ;     // [NS] K tiles
+  unsigned char *vt = kt + NS * C::kKv;                 // [NS] V tiles
+  TileShared &sh = *reinterpret_cast<TileShared *>(vt + NS * C::kKv);
+  const Layer &c = p.c;
+  const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  Share share;
+  if (!find_share<kTileRows, kTileKeys, kTileThreads>(p, g, sh.share, share)) return;
+  if (tid == 0) {
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.s_full[i], 2);  // the MMA thread's own arrival and its commit
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.pv_done[i], 1);
+      mbar_init(&sh.k_full[i], 4);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 4);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;  // columns: S0 0, S1 128, O0 256, O1 384
+  bool ok = true;
+  Entry en;
+  Piece pc;
+
+  if (warp < 8) {
+    // ================= softmax =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int q = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + (uint32_t)(q * 128), o_at = tmem + lanes + (uint32_t)(256 + q * 128);
+    int ns = 0;   // tiles this row tile has gone through
+    int nk = 0;   // key tiles of the block (slots of the scale ring)
+    // a wait that gave up (ok false) ends the products, not the loop: every
+    // warp reaches the same soft_sync barriers
+    while (next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+      const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
+      const int nr = en.r1 - en.r0;
+      const bool on = q * 128 < nr;          // this row tile has rows
+      const int r = en.r0 + q * 128 + row;   // row of the sequence
+      const bool mine = r < en.r1;
+      const int j = r / g.group, hq = pc.head * g.group + r - j * g.group;
+      const int pos = mine ? en.first + j : -1;
+      float m = -INFINITY, l = 0.0f;
+      if (on && nt > 0) {
+        unsigned char *hi = qs + q * C::kTerms * C::kQ + row * 16, *lo = hi + C::kQ;
+        float qf = 0.0f;
+        if (mine) {
+          qf = load_query<D, T>((const T *)p.q + (en.row0 + j) * p.q_row + hq * p.q_head, vec_q, p.scale, hi, lo);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 8; i++) {
+            *(uint4 *)(hi + i * 2048) = make_uint4(0, 0, 0, 0);
+            if (SPLIT) *(uint4 *)(lo + i * 2048) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.q_full[q]);
+        // positions of the row tile's first and last row
+        const int p_lo = en.first + (en.r0 + q * 128) / g.group;
+        const int p_hi = en.first + (min(en.r1, en.r0 + q * 128 + 128) - 1) / g.group;
+        for (int x = 0; x < nt && ok; x++, ns++) {
+          if (!warp_wait(&sh.s_full[q], (uint32_t)ns & 1u)) { ok = false; break; }
+          tc_fence_after();
+          uint32_t s[4][32];
+#pragma unroll
+          for (int i = 0; i < 4; i++) tc_ld<32>(s_at + 32 * i, s[i]);
+          const int slot = (nk + x) & 3;
+          const uint32_t live = sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
+          const int t0 = en.tile(pc.t0 + x) * kTileKeys;
+          const bool all = live == 0xffu && t0 + kTileKeys - 1 <= p_lo &&
+                           (p.window <= 0 || t0 > p_hi - p.window || t0 + kTileKeys - 1 < p.sinks);
+#pragma unroll
+          for (int i = 0; i < 4; i++) tc_wait_ld<32>(s[i]);
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+              for (int e = 0; e < 32; e++) {
+                const int tok = t0 + i * 32 + e;
+                const bool see = tok <= pos && (p.window <= 0 || tok > pos - p.window || tok < p.sinks) &&
+                                 ((live >> (i * 2 + e / 16)) & 1u);
+                if (!see) s[i][e] = 0xff800000u;  // -inf
+              }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 8; h++) {
+            float t = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; e++) t = fmaxf(t, __uint_as_float(s[h / 2][(h & 1) * 16 + e]));
+            top = fmaxf(top, t * fmaxf(sh.kf[slot][h] * qf, kTinyFactor) + sh.lv[slot][h]);
+          }
+          const bool grow = top > m + (x ? kTileSlack : 0.0f);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float now = grow ? top : m;
+            const float f = grow ? exp2_approx(m - now) : 1.0f;
+            m = now;
+            l *= f;
+            if (x) {  // every product into O before this tile's has completed (see the MMA warp)
+#pragma unroll 1
+              for (int i = 0; i < D / 32; i++) {
+                uint32_t o[32];
+                tc_ld<32>(o_at + 32 * i, o);
+                tc_wait_ld<32>(o);
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc_st32(o_at + 32 * i, o);
+              }
+            }
+          }
+          const float nm = m == -INFINITY ? 0.0f : -m;
+          const uint64_t nm2 = pack2(nm, nm);
+          uint64_t l2 = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t wh[16], wl[16];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const float f = fmaxf(sh.kf[slot][i * 2 + h] * qf, kTinyFactor), w = sh.wf[slot][i * 2 + h];
+              const uint64_t f2 = pack2(f, f), w2 = pack2(w, w);
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const int at = h * 16 + 2 * e;
+                const uint64_t a = ffma2((uint64_t)s[i][at] | ((uint64_t)s[i][at + 1] << 32), f2, nm2);
+                const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
+                l2 = fadd2(l2, b);
+                const uint64_t v = fmul2(b, w2);
+                const uint32_t pk = pack_h2(lo_of(v), hi_of(v));
+                wh[h * 8 + e] = pk;
+                if (SPLIT) {
+                  const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&pk));
+                  wl[h * 8 + e] = pack_h2(lo_of(v) - u.x, hi_of(v) - u.y);
+                }
+              }
+            }
+            // 32 keys: 16 columns of packed weights over the scores already read
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::
+                    "r"(wh[0]), "r"(wh[1]), "r"(wh[2]), "r"(wh[3]), "r"(wh[4]), "r"(wh[5]), "r"(wh[6]), "r"(wh[7]),
+                "r"(wh[8]), "r"(wh[9]), "r"(wh[10]), "r"(wh[11]), "r"(wh[12]), "r"(wh[13]), "r"(wh[14]), "r"(wh[15]),
+                "r"(s_at + 16 * i)
+                : "memory");
+            if (SPLIT)
+              asm volatile(
+                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::
+                      "r"(wl[0]), "r"(wl[1]), "r"(wl[2]), "r"(wl[3]), "r"(wl[4]), "r"(wl[5]), "r"(wl[6]), "r"(wl[7]),
+                  "r"(wl[8]), "r"(wl[9]), "r"(wl[10]), "r"(wl[11]), "r"(wl[12]), "r"(wl[13]), "r"(wl[14]), "r"(wl[15]),
+                  "r"(s_at + 64 + 16 * i)
+                  : "memory");
+          }
+          l += lo_of(l2) + hi_of(l2);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.p_full[q]);
+        }
+      }
+      nk += nt;
+      // ---- the piece's result ----
+      const int kPart = kTileRows * (D + 2);
+      float *part = g.parts + (int64_t)(pc.starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x) * kPart;
+      if (on && ok) {
+        if (nt > 0) {
+          if (!warp_wait(&sh.pv_done[q], (uint32_t)(ns - 1) & 1u)) ok = false;
+          tc_fence_after();
+        }
+        const int pr = q * 128 + row;  // row of the item
+        const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / (l * kTileShift)) : 1.0f;
+        T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
+#pragma unroll 1
+        for (int hf = 0; hf < D / 64; hf++) {
+          uint32_t o[2][32];
+          if (nt > 0) {
+            tc_ld<32>(o_at + 64 * hf, o[0]);
+            tc_ld<32>(o_at + 64 * hf + 32, o[1]);
+            tc_wait_ld<32>(o[0]);
+            tc_wait_ld<32>(o[1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[0][e] = o[1][e] = 0;
+          }
+          if (mine) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {  // elements 16 t .. 16 t + 15 of this half
+              float v[16];
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const int n = 8 * (e / 2) + 2 * t + (e & 1);
+                v[e] = __uint_as_float(o[n / 32][n % 32]) * inv;
+              }
+              const int d0 = hf * 64 + t * 16;
+              if (!pc.whole) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                  *(float4 *)(part + (int64_t)pr * D + d0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+              } else if (vec_o) {
+                constexpr int N = 16 / sizeof(T);
+#pragma unroll
+                for (int e = 0; e < 16; e += N) {
+                  uint4 w;
+                  T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+                  for (int u = 0; u < N; u++) x[u] = from_f32<T>(v[e + u]);
+                  *(uint4 *)(dst + d0 + e) = w;
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) dst[d0 + e] = from_f32<T>(v[e]);
+              }
+            }
+          }
+        }
+        if (mine) {
+          if (pc.whole) {
+            if (p.lse) p.lse[(en.row0 + j) * p.n_heads + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+          } else {
+            part[kTileRows * D + pr] = m;
+            part[kTileRows * D + kTileRows + pr] = l;
+          }
+        }
+        tc_fence_before();  // O has been read before the next piece's first product overwrites it
+      }
+      if (!pc.whole) {
+        // the block that finishes the item last joins its parts
+        __threadfence();
+        soft_sync();
+        if (tid == 0) {
+          const int done = atomicAdd(&g.count[pc.c0], 1);
+          sh.last = done == pc.parts - 1;
+          if (sh.last) g.count[pc.c0] = 0;
+        }
+        soft_sync();
+        if (sh.last) {
+          __threadfence();
+          constexpr int E = D / 32;
+          for (int rr = warp; rr < nr; rr += 8) {
+            float top = -INFINITY;
+            for (int k = lane; k < pc.parts; k += 32)
+              top = fmaxf(top, __ldcg(g.parts + (int64_t)part_slot(pc.c0, k) * kPart + kTileRows * D + rr));
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float sum = 0.0f, acc[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] = 0.0f;
+#pragma unroll 4
+            for (int k = 0; k < pc.parts; k++) {
+              const float *y = g.parts + (int64_t)part_slot(pc.c0, k) * kPart;
+              const float pm = __ldcg(y + kTileRows * D + rr), pl = __ldcg(y + kTileRows * D + kTileRows + rr);
+              const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - top);
+              sum += f * pl;
+#pragma unroll
+              for (int e = 0; e < E; e++) acc[e] += f * __ldcg(y + rr * D + e * 32 + lane);
+            }
+            const int r2 = en.r0 + rr, j2 = r2 / g.group, h2 = pc.head * g.group + r2 - j2 * g.group;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kTileShift);
+            T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head;
+#pragma unroll
+            for (int e = 0; e < E; e++) dst[e * 32 + lane] = from_f32<T>(acc[e] * inv);
+            if (p.lse && lane == 0)
+              p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+          }
+        }
+        soft_sync();  // sh.last is free
+      }
+    }
+  } else if (warp < 12) {
+    // ================= converters =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    const int w = warp - 8;
+    constexpr int HF = D / 64;
+    const int nblk = c.page / c.block;
+    int nk = 0;
+    while (ok && next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+      const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
+      if (nt == 0) continue;
+      const int32_t *trow = c.table + (int64_t)en.s * c.max_pages;
+      // this warp's tokens of a tile: groups 2 w and 2 w + 1
+      auto pages = [&](int x, int (&pid)[2]) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const int tok = en.tile(pc.t0 + x) * kTileKeys + w * 32 + u * 16;
+          const bool in = x < nt && tok <= en.p_hi &&
+                          (p.window <= 0 || tok + 15 > en.p_lo - p.window || tok < p.sinks);
+          const int id = in ? trow[page_of(c, tok)] : -1;
+          pid[u] = (unsigned)id < (unsigned)c.n_pages ? id : -1;
+          if (id >= c.n_pages && lane == 0) atomicOr(c.status, kBadPage);
+        }
+      };
+      auto base = [&](int x, int u, int pid) {  // the group's first row of codes
+        const int tok = en.tile(pc.t0 + x) * kTileKeys + w * 32 + u * 16;
+        return ((int64_t)pid * c.kv + pc.head) * c.page + tok - page_of(c, tok) * c.page;
+      };
+      uint4 kr[4][HF], vr[4][HF];
+      float ks = 1.0f, vs = 1.0f;  // lanes 0, 1: the scales of the warp's groups
+      auto load_k = [&](int x, const int (&pid)[2]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int id = pid[i >> 1];
+          if (id >= 0) {
+            const int8_t *src = c.k + (base(x, i >> 1, id) + (i & 1) * 8 + (lane & 7)) * D + (lane >> 3) * 16;
+#pragma unroll
+            for (int h = 0; h < HF; h++) kr[i][h] = __ldg((const uint4 *)(src + h * 64));
+          } else {
+#pragma unroll
+            for (int h = 0; h < HF; h++) kr[i][h] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        ks = vs = 1.0f;
+        if (lane < 2) {
+          const int id = lane ? pid[1] : pid[0];
+          if (id >= 0) {
+            const int tok = en.tile(pc.t0 + x) * kTileKeys + w * 32 + lane * 16;
+            const int slot = tok - page_of(c, tok) * c.page;
+            const int64_t at = ((int64_t)id * c.kv + pc.head) * nblk + slot / c.block;
+            ks = __ldg(c.ks + at);
+            vs = __ldg(c.vs + at);
+          }
+        }
+      };
+      auto load_v = [&](int x, const int (&pid)[2]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int id = pid[i >> 1];
+          if (id >= 0) {
+            const int8_t *src = c.v + (base(x, i >> 1, id) + (i & 1) * 8 + (lane >> 2)) * D + (lane & 3) * 16;
+#pragma unroll
+            for (int h = 0; h < HF; h++) vr[i][h] = __ldg((const uint4 *)(src + h * 64));
+          } else {
+#pragma unroll
+            for (int h = 0; h < HF; h++) vr[i][h] = make_uint4(0, 0, 0, 0);
+          }
+        }
+      };
+      int pid[2], nxt[2];
+      pages(0, pid);
+      load_k(0, pid);
+      load_v(0, pid);
+      pages(1, nxt);
+      for (int x = 0; x < nt; x++, nk++) {
+        const int st = nk % NS;
+        const uint32_t turn = (uint32_t)(nk / NS) & 1u;
+        if (!warp_wait(&sh.k_empty[st], turn ^ 1u)) { ok = false; break; }
+        unsigned char *kd = kt + st * C::kKv;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int h = 0; h < HF; h++) {
+            const uint32_t a[4] = {kr[i][h].x, kr[i][h].y, kr[i][h].z, kr[i][h].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t y = a[e] ^ 0x80808080u;
+              o[2 * e] = codes_f16(y, 0x4140);
+              o[2 * e + 1] = codes_f16(y, 0x4342);
+            }
+            const int tok = w * 32 + i * 8 + (lane & 7), kc = h * 8 + (lane >> 3) * 2;
+            *(uint4 *)(kd + (kc * 128 + tok) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+            *(uint4 *)(kd + ((kc + 1) * 128 + tok) * 16) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        const int slot = nk & 3;
+        if (lane < 2) {
+          const float v = vs > 0.0f ? vs : 1.0f;
+          sh.kf[slot][2 * w + lane] = ks > 0.0f ? ks : 1.0f;  // a scale of 0 has codes of 0
+          sh.lv[slot][2 * w + lane] = log2_approx(v);
+          sh.wf[slot][2 * w + lane] = v * kTileShift;
+        }
+        if (lane == 0) sh.live[slot][w] = ((pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u)) << (2 * w);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.k_full[st]);
+        if (x + 1 < nt) load_k(x + 1, nxt);
+        if (!warp_wait(&sh.v_empty[st], turn ^ 1u)) { ok = false; break; }
+        const uint32_t vd = smem_u32(vt + st * C::kKv);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int h = 0; h < HF; h++) {
+            const uint32_t a[4] = {vr[i][h].x, vr[i][h].y, vr[i][h].z, vr[i][h].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t y = a[e] ^ 0x80808080u;
+              o[2 * e] = codes_f16(y, 0x4140);
+              o[2 * e + 1] = codes_f16(y, 0x4342);
+            }
+            // matrices p = 0..3 then 4..7; lane gives the address of row (lane & 7) of matrix lane / 8
+            const uint32_t at = vd + (uint32_t)(((w * 4 + i) * D + h * 64 + (lane >> 3) * 8 + (lane & 7)) * 16);
+            stmatrix_t(at, o[0], o[1], o[2], o[3]);
+            stmatrix_t(at + 32 * 16, o[4], o[5], o[6], o[7]);
+          }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.v_full[st]);
+        if (x + 1 < nt) load_v(x + 1, nxt);
+        pid[0] = nxt[0];
+        pid[1] = nxt[1];
+        if (x + 2 < nt) pages(x + 2, nxt);
+      }
+    }
+  } else {
+    // ================= MMA =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 12 && lane == 0) {
+      const uint32_t id_s = umma_idesc_f16(128), id_o = umma_idesc_f16(D);
+      const uint64_t q0 = umma_desc(qs, 2048, 128), k0 = umma_desc(kt, 2048, 128), v0 = umma_desc(vt, D * 16, 128);
+      int nq[2] = {0, 0}, ns[2] = {0, 0}, np[2] = {0, 0}, nk = 0;
+      // S of row tile q from key tile stage st: when the last product that
+      // read its weights (they lie over the scores) has completed
+      auto scores = [&](int q, int st) {
+        if (np[q] > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np[q] - 1) & 1u)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < C::kTerms; t++)
+#pragma unroll
+          for (int i = 0; i < D / 16; i++)
+            tc_mma_f16(tmem + q * 128, q0 + (uint64_t)(((q * C::kTerms + t) * C::kQ + i * 4096) >> 4),
+                       k0 + (uint64_t)((st * C::kKv + i * 4096) >> 4), id_s, (uint32_t)(t | i));
+        mbar_arrive(&sh.s_full[q]);
+        tc_commit(&sh.s_full[q]);
+        ns[q]++;
+        return true;
+      };
+      while (ok && next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+        const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
+        if (nt == 0) continue;
+        const int tiles = en.r1 - en.r0 > 128 ? 2 : 1;
+        for (int x = -1; x < nt && ok; x++) {
+          // after O += W V of tile x (row tile q): S of tile x + 1
+          const int st = (nk + x) % NS, st1 = (nk + x + 1) % NS;
+          for (int q = 0; q < tiles && ok; q++) {
+            if (x >= 0) {
+              if (q == 0 && !mbar_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u)) { ok = false; break; }
+              if (!mbar_wait(&sh.p_full[q], (uint32_t)np[q] & 1u)) { ok = false; break; }
+              tc_fence_after();
+#pragma unroll
+              for (int t = 0; t < C::kTerms; t++)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                  tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + t * 64 + i * 8,
+                            v0 + (uint64_t)((st * C::kKv + i * 2 * D * 16) >> 4), id_o, (uint32_t)(x | t | i));
+              tc_commit(&sh.pv_done[q]);
+              np[q]++;
+              if (q == tiles - 1) tc_commit(&sh.v_empty[st]);
+            } else {
+              if (!mbar_wait(&sh.q_full[q], (uint32_t)nq[q] & 1u)) { ok = false; break; }
+              nq[q]++;
+            }
+            if (x + 1 < nt) {
+              if (q == 0 && !mbar_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u)) { ok = false; break; }
+              if (!scores(q, st1)) { ok = false; break; }
+              if (q == tiles - 1) tc_commit(&sh.k_empty[st1]);
+            }
+          }
+        }
+        nk += nt;
+      }
+      // every product completes before the tensor memory is released
+      for (int q = 0; q < 2; q++)
+        if (np[q] > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np[q] - 1) & 1u)) ok = false;
+    }
+    __syncwarp();
+  }
+  if (!ok && lane == 0) atomicOr(c.status, kWaitTimeout);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <int D, typename T>
+static int launch_tile(const AttendArgs &a, int sm_count, cudaStream_t st) {
+  using C = TileCfg<D, sizeof(T) == 4>;
+  WorkGrid g;
+  g.group = a.n_heads / a.c.kv;
+  g.per_seq = (int)ceil_div((int64_t)a.b.n * g.group, kTileRows);
+  g.entries = a.b.m * g.per_seq;
+  g.min_share = 2;
+  g.count = (int32_t *)a.ws;
+  g.parts = (float *)((char *)a.ws + kMaxBlocks * 4);
+  const bool vq = ((uintptr_t)a.q & 15) == 0 && a.q_row * sizeof(T) % 16 == 0 && a.q_head * sizeof(T) % 16 == 0;
+  const bool vo = ((uintptr_t)a.out & 15) == 0 && a.o_row * sizeof(T) % 16 == 0 && a.o_head * sizeof(T) % 16 == 0;
+  static std::atomic<size_t> limit[64];
+  const size_t bytes = C::kOperands + sizeof(TileShared);
+  const int rc = raise_smem_limit((const void *)attend_tile_kernel<D, T>, bytes, limit);
+  if (rc) return rc;
+  attend_tile_kernel<D, T><<<sm_count, kTileThreads, bytes, st>>>(a, g, vq, vo);
+  SC_CUDA(cudaGetLastError());
+  note_launch();
+  return kOk;
+}
+
+size_t tile_ws_bytes(int sm_count) { return (size_t)sm_count * 2 * kTileRows * 130 * 4; }
+
+int attend_tile(const AttendArgs &a, int sm_count, cudaStream_t st) {
+  const bool wide = a.head_dim == 128;
+  if (a.dtype == SC_DTYPE_F32) return wide ? launch_tile<128, float>(a, sm_count, st) : launch_tile<64, float>(a, sm_count, st);
+  if (a.dtype == SC_DTYPE_F16) return wide ? launch_tile<128, __half>(a, sm_count, st) : launch_tile<64, __half>(a, sm_count, st);
+  return wide ? launch_tile<128, __nv_bfloat16>(a, sm_count, st) : launch_tile<64, __nv_bfloat16>(a, sm_count, st);
+}
+
+}  // namespace kv8
+}  // namespace sc
