@@ -34,6 +34,7 @@ namespace kv8 {
 
 constexpr int kStepTile = 64;    // tokens per tile: 16 for each warp
 constexpr int kStepThreads = 128;
+constexpr int kStepOver = 1;
 constexpr float kShift = 256.0f;  // 2^8
 constexpr float kSlack = 7.0f;
 
@@ -98,11 +99,11 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
 
   Share share;
-  if (!find_share<ROWS, kStepTile, kStepThreads>(p, g, sh.share, share)) return;
+  if (!find_share<ROWS, kStepTile, kStepOver, kStepThreads>(p, g, sh.share, share)) return;
   Entry en;
   Piece pc;
   const int nblk = c.page / c.block;
-  while (next_piece<ROWS, kStepTile>(p, g, share, en, pc)) {
+  while (next_piece<ROWS, kStepTile, kStepOver>(p, g, share, en, pc)) {
     const int nr = en.r1 - en.r0;
     // ---- the rows of q: one warp a row ----
     for (int r = warp; r < ROWS; r += 4) {
@@ -448,7 +449,7 @@ static int launch_step(const AttendArgs &a, int sm_count, cudaStream_t st) {
   int64_t keys = a.max_len;
   if (a.window > 0 && (int64_t)a.window + a.b.n + a.sinks + 2 * kStepTile < keys)
     keys = (int64_t)a.window + a.b.n + a.sinks + 2 * kStepTile;
-  const int64_t most = ceil_div((ceil_div(keys, kStepTile) + 1) * g.entries * a.c.kv, g.min_share);
+  const int64_t most = ceil_div((ceil_div(keys, kStepTile) + 1 + kStepOver) * g.entries * a.c.kv, g.min_share);
   int64_t blocks = (int64_t)sm_count * (NT == 1 ? 4 : 3);
   if (most < blocks) blocks = most;
   if (blocks < 1) blocks = 1;

@@ -33,7 +33,8 @@ namespace sc {
 namespace kv8 {
 
 constexpr int kTileRows = 256, kTileKeys = 128;
-constexpr int kTileThreads = 512;  // 13 warps work; setmaxnreg needs whole warpgroups
+constexpr int kTileThreads = 416;
+constexpr int kTileOver = 3;  // an item's queries and result cost about as much as three tiles
 constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
 constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
 
@@ -103,19 +104,71 @@ __device__ __forceinline__ void stmatrix_t(uint32_t addr, uint32_t a, uint32_t b
                : "memory");
 }
 
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+
+// The lowest n bits.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+template <typename T>
+__device__ __forceinline__ void store16(T *dst, const float (&v)[16], int vec) {
+  if (vec) {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int e = 0; e < 16; e += N) {
+      uint4 w;
+      T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+      for (int u = 0; u < N; u++) x[u] = from_f32<T>(v[e + u]);
+      *(uint4 *)(dst + e) = w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e++) dst[e] = from_f32<T>(v[e]);
+  }
+}
+
 // A row of q as f16 (hi and, for f32, lo), scaled by a power of two with the
 // sign of the score factor; returns the factor of its scores.
 template <int D, typename T>
 __device__ __forceinline__ float load_query(const T *src, bool vec, float scale, unsigned char *hi, unsigned char *lo) {
   constexpr int N = 16 / sizeof(T);  // elements of a 16-byte load
+  constexpr bool kKeep = sizeof(T) == 2;  // a row fits the registers: read once
+  uint4 raw[kKeep ? D / N : 1];
   float top = 0.0f;
   if (vec) {
-#pragma unroll 8
-    for (int i = 0; i < D / N; i++) {
-      const uint4 w = __ldg((const uint4 *)src + i);
-      const T *x = reinterpret_cast<const T *>(&w);
+    if constexpr (kKeep) {
 #pragma unroll
-      for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+      for (int i = 0; i < D / N; i++) raw[i] = __ldg((const uint4 *)src + i);
+#pragma unroll
+      for (int i = 0; i < D / N; i++) {
+        const T *x = reinterpret_cast<const T *>(&raw[i]);
+#pragma unroll
+        for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+      }
+    } else {
+#pragma unroll 16
+      for (int i = 0; i < D / N; i++) {
+        const uint4 w = __ldg((const uint4 *)src + i);
+        const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+      }
+    }
+  } else if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < D / N; i++) {
+      T *x = reinterpret_cast<T *>(&raw[i]);
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        x[e] = src[i * N + e];
+        top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+      }
     }
   } else {
 #pragma unroll 8
@@ -128,16 +181,21 @@ __device__ __forceinline__ float load_query(const T *src, bool vec, float scale,
   // score factors stay positive: a group's largest score is its largest product
   if (scale < 0.0f) up = -up;
   if (scale == 0.0f) up = 0.0f;
-#pragma unroll 4
+#pragma unroll(kKeep ? 16 : 4)
   for (int i = 0; i < D / 8; i++) {
     float x[8];
-    if (vec) {
+    if constexpr (kKeep) {
+      const T *y = reinterpret_cast<const T *>(&raw[i]);
 #pragma unroll
-      for (int j = 0; j < 8 / N; j++) {
-        const uint4 w = __ldg((const uint4 *)src + i * (8 / N) + j);
-        const T *y = reinterpret_cast<const T *>(&w);
+      for (int e = 0; e < 8; e++) x[e] = to_f32<T>(y[e]) * up;
+    } else if (vec) {
 #pragma unroll
-        for (int e = 0; e < N; e++) x[j * N + e] = to_f32<T>(y[e]) * up;
+      for (int j = 0; j < 2; j++) {
+        const float4 w = __ldg((const float4 *)src + i * 2 + j);
+        x[4 * j] = w.x * up;
+        x[4 * j + 1] = w.y * up;
+        x[4 * j + 2] = w.z * up;
+        x[4 * j + 3] = w.w * up;
       }
     } else {
 #pragma unroll
@@ -173,7 +231,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   Share share;
-  if (!find_share<kTileRows, kTileKeys, kTileThreads>(p, g, sh.share, share)) return;
+  if (!find_share<kTileRows, kTileKeys, kTileOver, kTileThreads>(p, g, sh.share, share)) return;
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.q_full[i], 4);
@@ -202,7 +260,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (warp < 8) {
     // ================= softmax =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int q = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + (uint32_t)(q * 128), o_at = tmem + lanes + (uint32_t)(256 + q * 128);
@@ -210,7 +267,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     int nk = 0;   // key tiles of the block (slots of the scale ring)
     // a wait that gave up (ok false) ends the products, not the loop: every
     // warp reaches the same soft_sync barriers
-    while (next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+    while (next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
       const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
       const int nr = en.r1 - en.r0;
       const bool on = q * 128 < nr;          // this row tile has rows
@@ -240,34 +297,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int x = 0; x < nt && ok; x++, ns++) {
           if (!warp_wait(&sh.s_full[q], (uint32_t)ns & 1u)) { ok = false; break; }
           tc_fence_after();
-          uint32_t s[4][32];
-#pragma unroll
-          for (int i = 0; i < 4; i++) tc_ld<32>(s_at + 32 * i, s[i]);
           const int slot = (nk + x) & 3;
           const uint32_t live = sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
           const int t0 = en.tile(pc.t0 + x) * kTileKeys;
           const bool all = live == 0xffu && t0 + kTileKeys - 1 <= p_lo &&
                            (p.window <= 0 || t0 > p_hi - p.window || t0 + kTileKeys - 1 < p.sinks);
+          // Hides what the row does not see of columns c .. c + 31.
+          auto hide = [&](uint32_t (&s)[32], int c0) {
+            const int d = pos - t0 - c0 + 1;
+            uint32_t see = below(d);
+            if (p.window > 0) see &= ~below(d - p.window) | below(p.sinks - t0 - c0);
+            const uint32_t lv = live >> (c0 >> 4);
+            see &= (lv & 1u ? 0xffffu : 0u) | (lv & 2u ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int i = 0; i < 4; i++) tc_wait_ld<32>(s[i]);
-          if (!all) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-              for (int e = 0; e < 32; e++) {
-                const int tok = t0 + i * 32 + e;
-                const bool see = tok <= pos && (p.window <= 0 || tok > pos - p.window || tok < p.sinks) &&
-                                 ((live >> (i * 2 + e / 16)) & 1u);
-                if (!see) s[i][e] = 0xff800000u;  // -inf
-              }
-          }
+            for (int e = 0; e < 32; e++)
+              if (!((see >> e) & 1u)) s[e] = 0xff800000u;  // -inf
+          };
+          // The scores are read twice, 64 columns at a time: all 128 in
+          // registers cost spills, and unrolled four times as much code, more
+          // than the SM's instruction cache holds for its four roles.
           float top = -INFINITY;
+#pragma unroll 1
+          for (int i = 0; i < 4; i += 2) {
+            uint32_t s[2][32];
+            tc_ld<32>(s_at + 32 * i, s[0]);
+            tc_ld<32>(s_at + 32 * i + 32, s[1]);
+            tc_wait_ld<32>(s[0]);
+            tc_wait_ld<32>(s[1]);
+            if (!all) {
+              hide(s[0], 32 * i);
+              hide(s[1], 32 * i + 32);
+            }
 #pragma unroll
-          for (int h = 0; h < 8; h++) {
-            float t = -INFINITY;
+            for (int h = 0; h < 4; h++) {
+              float t = __uint_as_float(s[h / 2][(h & 1) * 16]);
 #pragma unroll
-            for (int e = 0; e < 16; e++) t = fmaxf(t, __uint_as_float(s[h / 2][(h & 1) * 16 + e]));
-            top = fmaxf(top, t * fmaxf(sh.kf[slot][h] * qf, kTinyFactor) + sh.lv[slot][h]);
+              for (int e = 1; e < 16; e++) t = fmaxf(t, __uint_as_float(s[h / 2][(h & 1) * 16 + e]));
+              top = fmaxf(top, t * fmaxf(sh.kf[slot][2 * i + h] * qf, kTinyFactor) + sh.lv[slot][2 * i + h]);
+            }
           }
           const bool grow = top > m + (x ? kTileSlack : 0.0f);
           if (__any_sync(0xffffffffu, grow)) {
@@ -290,42 +357,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const float nm = m == -INFINITY ? 0.0f : -m;
           const uint64_t nm2 = pack2(nm, nm);
           uint64_t l2 = 0;
+#pragma unroll 1
+          for (int i = 0; i < 4; i += 2) {
+            uint32_t s[2][32];
+            tc_ld<32>(s_at + 32 * i, s[0]);
+            tc_ld<32>(s_at + 32 * i + 32, s[1]);
+            tc_wait_ld<32>(s[0]);
+            tc_wait_ld<32>(s[1]);
+            if (!all) {
+              hide(s[0], 32 * i);
+              hide(s[1], 32 * i + 32);
+            }
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t wh[16], wl[16];
+            for (int u = 0; u < 2; u++) {
+              // 32 keys: 16 columns of packed weights (and 16 of their low
+              // terms) over the scores just read
+              uint32_t w[32];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const float f = fmaxf(sh.kf[slot][i * 2 + h] * qf, kTinyFactor), w = sh.wf[slot][i * 2 + h];
-              const uint64_t f2 = pack2(f, f), w2 = pack2(w, w);
+              for (int h = 0; h < 2; h++) {
+                const int gr = 2 * (i + u) + h;
+                const float f = fmaxf(sh.kf[slot][gr] * qf, kTinyFactor), wf = sh.wf[slot][gr];
+                const uint64_t f2 = pack2(f, f), w2 = pack2(wf, wf);
 #pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const int at = h * 16 + 2 * e;
-                const uint64_t a = ffma2((uint64_t)s[i][at] | ((uint64_t)s[i][at + 1] << 32), f2, nm2);
-                const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
-                l2 = fadd2(l2, b);
-                const uint64_t v = fmul2(b, w2);
-                const uint32_t pk = pack_h2(lo_of(v), hi_of(v));
-                wh[h * 8 + e] = pk;
-                if (SPLIT) {
-                  const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&pk));
-                  wl[h * 8 + e] = pack_h2(lo_of(v) - u.x, hi_of(v) - u.y);
+                for (int e = 0; e < 8; e++) {
+                  const int at = h * 16 + 2 * e;
+                  const uint64_t a = ffma2((uint64_t)s[u][at] | ((uint64_t)s[u][at + 1] << 32), f2, nm2);
+                  const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
+                  l2 = fadd2(l2, b);
+                  const uint64_t v = fmul2(b, w2);
+                  const uint32_t pk = pack_h2(lo_of(v), hi_of(v));
+                  w[h * 8 + e] = pk;
+                  if (SPLIT) {
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&pk));
+                    w[16 + h * 8 + e] = pack_h2(lo_of(v) - y.x, hi_of(v) - y.y);
+                  }
                 }
               }
+              if constexpr (SPLIT) {
+                tc_st32(s_at + 32 * (i + u), w);
+              } else {
+                tc_st16(s_at + 32 * (i + u), w);
+              }
             }
-            // 32 keys: 16 columns of packed weights over the scores already read
-            asm volatile(
-                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::
-                    "r"(wh[0]), "r"(wh[1]), "r"(wh[2]), "r"(wh[3]), "r"(wh[4]), "r"(wh[5]), "r"(wh[6]), "r"(wh[7]),
-                "r"(wh[8]), "r"(wh[9]), "r"(wh[10]), "r"(wh[11]), "r"(wh[12]), "r"(wh[13]), "r"(wh[14]), "r"(wh[15]),
-                "r"(s_at + 16 * i)
-                : "memory");
-            if (SPLIT)
-              asm volatile(
-                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::
-                      "r"(wl[0]), "r"(wl[1]), "r"(wl[2]), "r"(wl[3]), "r"(wl[4]), "r"(wl[5]), "r"(wl[6]), "r"(wl[7]),
-                  "r"(wl[8]), "r"(wl[9]), "r"(wl[10]), "r"(wl[11]), "r"(wl[12]), "r"(wl[13]), "r"(wl[14]), "r"(wl[15]),
-                  "r"(s_at + 64 + 16 * i)
-                  : "memory");
           }
           l += lo_of(l2) + hi_of(l2);
           tc_wait_st();
@@ -372,19 +445,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 16; e += 4)
                   *(float4 *)(part + (int64_t)pr * D + d0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-              } else if (vec_o) {
-                constexpr int N = 16 / sizeof(T);
-#pragma unroll
-                for (int e = 0; e < 16; e += N) {
-                  uint4 w;
-                  T *x = reinterpret_cast<T *>(&w);
-#pragma unroll
-                  for (int u = 0; u < N; u++) x[u] = from_f32<T>(v[e + u]);
-                  *(uint4 *)(dst + d0 + e) = w;
-                }
               } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) dst[d0 + e] = from_f32<T>(v[e]);
+                store16<T>(dst + d0, v, vec_o);
               }
             }
           }
@@ -411,31 +473,36 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         soft_sync();
         if (sh.last) {
           __threadfence();
-          constexpr int E = D / 32;
-          for (int rr = warp; rr < nr; rr += 8) {
-            float top = -INFINITY;
-            for (int k = lane; k < pc.parts; k += 32)
+          // a thread joins 16 elements of a row
+          for (int u = tid; u < nr * (D / 16); u += 256) {
+            const int rr = u / (D / 16), d0 = u % (D / 16) * 16;
+            float top = -INFINITY, sum = 0.0f, acc[16];
+            for (int k = 0; k < pc.parts; k++)
               top = fmaxf(top, __ldcg(g.parts + (int64_t)part_slot(pc.c0, k) * kPart + kTileRows * D + rr));
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float sum = 0.0f, acc[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) acc[e] = 0.0f;
-#pragma unroll 4
+            for (int e = 0; e < 16; e++) acc[e] = 0.0f;
+#pragma unroll 2
             for (int k = 0; k < pc.parts; k++) {
               const float *y = g.parts + (int64_t)part_slot(pc.c0, k) * kPart;
               const float pm = __ldcg(y + kTileRows * D + rr), pl = __ldcg(y + kTileRows * D + kTileRows + rr);
               const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - top);
               sum += f * pl;
 #pragma unroll
-              for (int e = 0; e < E; e++) acc[e] += f * __ldcg(y + rr * D + e * 32 + lane);
+              for (int e = 0; e < 4; e++) {
+                const float4 v = __ldcg((const float4 *)(y + rr * D + d0) + e);
+                acc[4 * e] += f * v.x;
+                acc[4 * e + 1] += f * v.y;
+                acc[4 * e + 2] += f * v.z;
+                acc[4 * e + 3] += f * v.w;
+              }
             }
             const int r2 = en.r0 + rr, j2 = r2 / g.group, h2 = pc.head * g.group + r2 - j2 * g.group;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kTileShift);
-            T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head;
+            T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
-            for (int e = 0; e < E; e++) dst[e * 32 + lane] = from_f32<T>(acc[e] * inv);
-            if (p.lse && lane == 0)
+            for (int e = 0; e < 16; e++) acc[e] *= inv;
+            store16<T>(dst, acc, vec_o);
+            if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
           }
         }
@@ -444,12 +511,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp < 12) {
     // ================= converters =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int w = warp - 8;
     constexpr int HF = D / 64;
     const int nblk = c.page / c.block;
     int nk = 0;
-    while (ok && next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+    while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
       const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
       if (nt == 0) continue;
       const int32_t *trow = c.table + (int64_t)en.s * c.max_pages;
@@ -578,8 +644,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else {
     // ================= MMA =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 12 && lane == 0) {
+    if (lane == 0) {
       const uint32_t id_s = umma_idesc_f16(128), id_o = umma_idesc_f16(D);
       const uint64_t q0 = umma_desc(qs, 2048, 128), k0 = umma_desc(kt, 2048, 128), v0 = umma_desc(vt, D * 16, 128);
       int nq[2] = {0, 0}, ns[2] = {0, 0}, np[2] = {0, 0}, nk = 0;
@@ -592,14 +657,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int t = 0; t < C::kTerms; t++)
 #pragma unroll
           for (int i = 0; i < D / 16; i++)
-            tc_mma_f16(tmem + q * 128, q0 + (uint64_t)(((q * C::kTerms + t) * C::kQ + i * 4096) >> 4),
+            tc_mma_f16(tmem + q * 128,
+                       q0 + (uint64_t)(((q * C::kTerms + C::kTerms - 1 - t) * C::kQ + i * 4096) >> 4),
                        k0 + (uint64_t)((st * C::kKv + i * 4096) >> 4), id_s, (uint32_t)(t | i));
         mbar_arrive(&sh.s_full[q]);
         tc_commit(&sh.s_full[q]);
         ns[q]++;
         return true;
       };
-      while (ok && next_piece<kTileRows, kTileKeys>(p, g, share, en, pc)) {
+      while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
         const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
         if (nt == 0) continue;
         const int tiles = en.r1 - en.r0 > 128 ? 2 : 1;
@@ -615,7 +681,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               for (int t = 0; t < C::kTerms; t++)
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                  tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + t * 64 + i * 8,
+                  tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + (i >> 1) * 32 + t * 16 + (i & 1) * 8,
                             v0 + (uint64_t)((st * C::kKv + i * 2 * D * 16) >> 4), id_o, (uint32_t)(x | t | i));
               tc_commit(&sh.pv_done[q]);
               np[q]++;

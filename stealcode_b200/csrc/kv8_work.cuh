@@ -5,7 +5,8 @@
 // head of that kv head), token-major; an item is ROWS of them, and its keys
 // are the tiles of TILE consecutive tokens that hold a token some row sees:
 // tiles [0, a) of the first `sinks` tokens, then tiles [b, c) of the window.
-// All items' tiles, one after the other, are cut into equal contiguous
+// Every item counts OVER units (its queries, its result) and one for each
+// tile; all items' units, one after the other, are cut into equal contiguous
 // shares, one per block, whatever the sequences' lengths: a block computes
 // whole items and at most two parts of items (the end of one, the start of
 // another).  Parts go to the workspace; the block that finishes an item last
@@ -21,7 +22,7 @@ struct WorkGrid {
   int group;       // query heads per kv head
   int per_seq;     // items per sequence and kv head, at most
   int entries;     // m * per_seq
-  int min_share;   // tiles; fewer blocks work when there are few tiles
+  int min_share;   // units; fewer blocks work when there are few
   int32_t *count;  // [blocks] parts done of the item that starts in a block
   float *parts;    // [2 * blocks] parts
 };
@@ -34,7 +35,7 @@ struct Entry {
   int p_lo, p_hi;   // positions of the first and the last row
   int a, b, c;
   __device__ __forceinline__ int tiles() const { return a + c - b; }
-  __device__ __forceinline__ int cost() const { return max(1, tiles()); }
+  __device__ __forceinline__ int steps() const { return max(1, tiles()); }  // an item without keys has a result too
   __device__ __forceinline__ int tile(int x) const { return x < a ? x : b + x - a; }
 };
 
@@ -64,15 +65,15 @@ __device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g
   return true;
 }
 
-// A block's share [pos, end) of all tiles and the entry that holds pos.
+// A block's share [pos, end) of all units and the entry that holds pos.
 struct Share {
   int64_t pos, end, total;
   int blocks;       // blocks that have a share
   int e;            // entry
-  int64_t at;       // first tile of entry e
+  int64_t at;       // first unit of entry e
 };
 
-// First block of `blocks` whose share reaches past tile `pos`.
+// The block whose share holds unit `pos`.
 __device__ __forceinline__ int block_of(int64_t pos, int64_t total, int blocks) {
   return (int)(((pos + 1) * blocks - 1) / total);
 }
@@ -84,7 +85,7 @@ struct ShareScratch {
 };
 
 // All threads of the block call; false when the block has nothing to do.
-template <int ROWS, int TILE, int THREADS>
+template <int ROWS, int TILE, int OVER, int THREADS>
 __device__ bool find_share(const AttendArgs &p, const WorkGrid &g, ShareScratch &sh, Share &o) {
   const int tid = (int)threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (g.entries + THREADS - 1) / THREADS;
@@ -92,7 +93,7 @@ __device__ bool find_share(const AttendArgs &p, const WorkGrid &g, ShareScratch 
   int64_t mine = 0;
   Entry en;
   for (int e = e0; e < e1; e++)
-    if (get_entry<ROWS, TILE>(p, g, e, en)) mine += (int64_t)en.cost() * p.c.kv;
+    if (get_entry<ROWS, TILE>(p, g, e, en)) mine += (int64_t)(OVER + en.steps()) * p.c.kv;
   int64_t x = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -118,7 +119,7 @@ __device__ bool find_share(const AttendArgs &p, const WorkGrid &g, ShareScratch 
     int64_t at = start;
     for (int e = e0; e < e1; e++) {
       if (!get_entry<ROWS, TILE>(p, g, e, en)) continue;
-      const int64_t n = (int64_t)en.cost() * p.c.kv;
+      const int64_t n = (int64_t)(OVER + en.steps()) * p.c.kv;
       if (o.pos < at + n) {
         sh.e = e;
         sh.at = at;
@@ -141,32 +142,37 @@ struct Piece {
   int c0, parts;       // block in which the item starts, and its parts
 };
 
-// Moves to the share's next piece (entry in `en`); false at its end.
-template <int ROWS, int TILE>
+// Moves to the share's next piece (entry in `en`); false at its end.  Tile t
+// of an item is unit OVER + t: a share that holds only the first OVER units
+// of an item has no piece of it.
+template <int ROWS, int TILE, int OVER>
 __device__ __forceinline__ bool next_piece(const AttendArgs &p, const WorkGrid &g, Share &o, Entry &en, Piece &q) {
-  if (o.pos >= o.end) return false;
-  while (true) {
+  while (o.pos < o.end) {
     if (!get_entry<ROWS, TILE>(p, g, o.e, en)) {
       o.e = (en.i + 1) * g.per_seq;  // the sequence has no more rows
       continue;
     }
-    const int64_t n = (int64_t)en.cost() * p.c.kv;
-    if (o.pos < o.at + n) break;
-    o.at += n;
-    o.e++;
+    const int steps = en.steps(), cost = OVER + steps;
+    const int64_t n = (int64_t)cost * p.c.kv;
+    if (o.pos >= o.at + n) {
+      o.at += n;
+      o.e++;
+      continue;
+    }
+    q.head = (int)((o.pos - o.at) / cost);
+    const int64_t s0 = o.at + (int64_t)q.head * cost + OVER;  // unit of tile 0
+    const int64_t end = o.end < s0 + steps ? o.end : s0 + steps;
+    q.t0 = o.pos > s0 ? (int)(o.pos - s0) : 0;
+    q.t1 = (int)(end - s0);
+    o.pos = end;
+    if (q.t1 <= q.t0) continue;
+    q.starts = q.t0 == 0;
+    q.whole = q.starts && q.t1 == steps;
+    q.c0 = q.starts ? (int)blockIdx.x : block_of(s0, o.total, o.blocks);
+    q.parts = (q.t1 == steps ? (int)blockIdx.x : block_of(s0 + steps - 1, o.total, o.blocks)) - q.c0 + 1;
+    return true;
   }
-  const int cost = en.cost();
-  const int64_t off = o.pos - o.at;
-  q.head = (int)(off / cost);
-  q.t0 = (int)(off - (int64_t)q.head * cost);
-  q.t1 = (int)min((int64_t)cost, q.t0 + (o.end - o.pos));
-  const int64_t s0 = o.pos - q.t0;
-  o.pos += q.t1 - q.t0;
-  q.starts = q.t0 == 0;
-  q.whole = q.starts && q.t1 == cost;
-  q.c0 = q.starts ? (int)blockIdx.x : block_of(s0, o.total, o.blocks);
-  q.parts = q.t1 == cost ? (int)blockIdx.x - q.c0 + 1 : block_of(s0 + cost - 1, o.total, o.blocks) - q.c0 + 1;
-  return true;
+  return false;
 }
 
 // Workspace slot of part k of the item that starts in block c0.
