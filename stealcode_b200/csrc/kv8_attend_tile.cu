@@ -5,15 +5,15 @@
 //
 // A block takes 256 rows (token, query head of the group) as two tiles of 128
 // and walks the keys 128 at a time:
-//   warps 0-3, 4-7  softmax of row tile 0, 1: a thread holds one row, reads
-//                   its 128 scores from tensor memory, writes the weights
-//                   back over them as f16, and rescales the output
+//   warps 0-7, 8-15 softmax of row tile 0, 1: two threads hold a row, read 64
+//                   of its scores each from tensor memory, write the weights
+//                   back over them as f16, and rescale the output
 //                   accumulator when its maximum has grown by more than 2^7;
-//   warps 8-11      read the codes of K and V (16-byte loads, one tile ahead
+//   warps 16-19     read the codes of K and V (16-byte loads, one tile ahead
 //                   in registers) and write them to shared memory as f16
 //                   operands: K as it lies (its depth is contiguous), V
 //                   transposed by stmatrix;
-//   warp 12         issues S = Q K^T and O += W V; while one row tile is in
+//   warp 20         issues S = Q K^T and O += W V; while one row tile is in
 //                   its softmax the other's products run.
 // The codes pass through the converters once for 256 rows, so their cost is
 // shared by all query heads of the group.
@@ -33,7 +33,7 @@ namespace sc {
 namespace kv8 {
 
 constexpr int kTileRows = 256, kTileKeys = 128;
-constexpr int kTileThreads = 416;
+constexpr int kTileThreads = 768;  // 21 warps work; setmaxnreg takes whole warpgroups
 constexpr int kTileOver = 3;  // an item's queries and result cost about as much as three tiles
 constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
 constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
@@ -55,13 +55,22 @@ struct TileShared {  // after the operands
   // written again only after both softmaxes have read it
   float kf[4][8], lv[4][8], wf[4][8];
   uint32_t live[4][4];  // two bits from each converter warp
+  float top[2][2][2][128];  // [tile parity][row tile][half][row]: largest score, and once a piece the sums
   ShareScratch share;
   uint32_t tmem;
   int last;
 };
 
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+
+// The two warps that hold the halves of 32 rows.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 __device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -115,65 +124,58 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
 // The lowest n bits.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
-template <typename T>
-__device__ __forceinline__ void store16(T *dst, const float (&v)[16], int vec) {
+// N consecutive elements (8 or 16) of a result row.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(T *dst, const float (&v)[N], int vec) {
   if (vec) {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int W = 16 / sizeof(T);
 #pragma unroll
-    for (int e = 0; e < 16; e += N) {
+    for (int e = 0; e < N; e += W) {
       uint4 w;
       T *x = reinterpret_cast<T *>(&w);
 #pragma unroll
-      for (int u = 0; u < N; u++) x[u] = from_f32<T>(v[e + u]);
+      for (int u = 0; u < W; u++) x[u] = from_f32<T>(v[e + u]);
       *(uint4 *)(dst + e) = w;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 16; e++) dst[e] = from_f32<T>(v[e]);
+    for (int e = 0; e < N; e++) dst[e] = from_f32<T>(v[e]);
   }
 }
 
-// A row of q as f16 (hi and, for f32, lo), scaled by a power of two with the
-// sign of the score factor; returns the factor of its scores.
+// 8 rows of q as f16 (hi and, for f32, lo), each scaled by a power of two
+// with the sign of the score factor.  Lane = (row of the 8, one of 4 16-byte
+// pieces): every load takes 64 contiguous bytes of a row, and every store 8
+// consecutive rows of an operand chunk, which share no bank.  src: the lane's
+// row, or nullptr (zeros).  Writes the row's score factor to *factor.
 template <int D, typename T>
-__device__ __forceinline__ float load_query(const T *src, bool vec, float scale, unsigned char *hi, unsigned char *lo) {
-  constexpr int N = 16 / sizeof(T);  // elements of a 16-byte load
-  constexpr bool kKeep = sizeof(T) == 2;  // a row fits the registers: read once
-  uint4 raw[kKeep ? D / N : 1];
-  float top = 0.0f;
-  if (vec) {
-    if constexpr (kKeep) {
+__device__ __forceinline__ void load_queries(const T *src, bool vec, float scale, unsigned char *hi, unsigned char *lo,
+                                             float *factor) {
+  constexpr int N = 16 / sizeof(T), S = D / (4 * N);  // elements of a piece, 64-byte segments of a row
+  const int piece = (threadIdx.x >> 3) & 3;
+  uint4 raw[S];
 #pragma unroll
-      for (int i = 0; i < D / N; i++) raw[i] = __ldg((const uint4 *)src + i);
+  for (int i = 0; i < S; i++) {
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (src && vec) raw[i] = __ldg((const uint4 *)src + i * 4 + piece);
+  }
+  if (src && !vec) {
 #pragma unroll
-      for (int i = 0; i < D / N; i++) {
-        const T *x = reinterpret_cast<const T *>(&raw[i]);
-#pragma unroll
-        for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
-      }
-    } else {
-#pragma unroll 16
-      for (int i = 0; i < D / N; i++) {
-        const uint4 w = __ldg((const uint4 *)src + i);
-        const T *x = reinterpret_cast<const T *>(&w);
-#pragma unroll
-        for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
-      }
-    }
-  } else if constexpr (kKeep) {
-#pragma unroll
-    for (int i = 0; i < D / N; i++) {
+    for (int i = 0; i < S; i++) {
       T *x = reinterpret_cast<T *>(&raw[i]);
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        x[e] = src[i * N + e];
-        top = fmaxf(top, fabsf(to_f32<T>(x[e])));
-      }
+      for (int e = 0; e < N; e++) x[e] = src[(i * 4 + piece) * N + e];
     }
-  } else {
-#pragma unroll 8
-    for (int i = 0; i < D; i++) top = fmaxf(top, fabsf(to_f32<T>(src[i])));
   }
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < S; i++) {
+    const T *x = reinterpret_cast<const T *>(&raw[i]);
+#pragma unroll
+    for (int e = 0; e < N; e++) top = fmaxf(top, fabsf(to_f32<T>(x[e])));
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
   int k = 0;
   if (top > 0.0f) k = min(100, 140 - (int)(__float_as_uint(top) >> 23));
   float up = __uint_as_float((uint32_t)(127 + k) << 23);
@@ -181,39 +183,29 @@ __device__ __forceinline__ float load_query(const T *src, bool vec, float scale,
   // score factors stay positive: a group's largest score is its largest product
   if (scale < 0.0f) up = -up;
   if (scale == 0.0f) up = 0.0f;
-#pragma unroll(kKeep ? 16 : 4)
-  for (int i = 0; i < D / 8; i++) {
-    float x[8];
-    if constexpr (kKeep) {
-      const T *y = reinterpret_cast<const T *>(&raw[i]);
+  if (piece == 0) *factor = fabsf(scale) * kLog2e * down;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = to_f32<T>(y[e]) * up;
-    } else if (vec) {
+  for (int i = 0; i < S; i++) {
+    const T *x = reinterpret_cast<const T *>(&raw[i]);
+    if constexpr (sizeof(T) == 2) {  // 8 elements: a chunk's row
+      uint32_t h[4];
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const float4 w = __ldg((const float4 *)src + i * 2 + j);
-        x[4 * j] = w.x * up;
-        x[4 * j + 1] = w.y * up;
-        x[4 * j + 2] = w.z * up;
-        x[4 * j + 3] = w.w * up;
+      for (int e = 0; e < 4; e++) h[e] = pack_h2(to_f32<T>(x[2 * e]) * up, to_f32<T>(x[2 * e + 1]) * up);
+      *(uint4 *)(hi + (i * 4 + piece) * 2048) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {  // 4 elements: half of it
+      uint32_t h[2], l[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float a = to_f32<T>(x[2 * e]) * up, b = to_f32<T>(x[2 * e + 1]) * up;
+        h[e] = pack_h2(a, b);
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
+        l[e] = pack_h2(a - y.x, b - y.y);
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = to_f32<T>(src[i * 8 + e]) * up;
+      const int at = (i * 2 + (piece >> 1)) * 2048 + (piece & 1) * 8;
+      *(uint2 *)(hi + at) = make_uint2(h[0], h[1]);
+      *(uint2 *)(lo + at) = make_uint2(l[0], l[1]);
     }
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      h[e] = pack_h2(x[2 * e], x[2 * e + 1]);
-      if (sizeof(T) == 4) {
-        const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
-        l[e] = pack_h2(x[2 * e] - b.x, x[2 * e + 1] - b.y);
-      }
-    }
-    *(uint4 *)(hi + i * 2048) = make_uint4(h[0], h[1], h[2], h[3]);
-    if (sizeof(T) == 4) *(uint4 *)(lo + i * 2048) = make_uint4(l[0], l[1], l[2], l[3]);
   }
-  return fabsf(scale) * kLog2e * down;
 }
 
 template <int D, typename T>
@@ -234,9 +226,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (!find_share<kTileRows, kTileKeys, kTileOver, kTileThreads>(p, g, sh.share, share)) return;
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sh.q_full[i], 4);
+      mbar_init(&sh.q_full[i], 8);
       mbar_init(&sh.s_full[i], 2);  // the MMA thread's own arrival and its commit
-      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_full[i], 8);
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.k_full[i], 4);
       mbar_init(&sh.k_empty[i], 1);
@@ -245,7 +237,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 20) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -258,15 +250,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   Entry en;
   Piece pc;
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ================= softmax =================
-    const int q = warp >> 2, row = tid & 127;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int q = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    const int pair = 2 + q * 4 + (warp & 3);  // named barrier of this warp and the one with the rows' other half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + (uint32_t)(q * 128), o_at = tmem + lanes + (uint32_t)(256 + q * 128);
+    const uint32_t s_at = tmem + lanes + (uint32_t)(q * 128 + half * 64), o_at = tmem + lanes + (uint32_t)(256 + q * 128);
     int ns = 0;   // tiles this row tile has gone through
     int nk = 0;   // key tiles of the block (slots of the scale ring)
     // a wait that gave up (ok false) ends the products, not the loop: every
-    // warp reaches the same soft_sync barriers
+    // warp reaches the same barriers
     while (next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
       const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
       const int nr = en.r1 - en.r0;
@@ -277,65 +271,71 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int pos = mine ? en.first + j : -1;
       float m = -INFINITY, l = 0.0f;
       if (on && nt > 0) {
-        unsigned char *hi = qs + q * C::kTerms * C::kQ + row * 16, *lo = hi + C::kQ;
-        float qf = 0.0f;
-        if (mine) {
-          qf = load_query<D, T>((const T *)p.q + (en.row0 + j) * p.q_row + hq * p.q_head, vec_q, p.scale, hi, lo);
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 8; i++) {
-            *(uint4 *)(hi + i * 2048) = make_uint4(0, 0, 0, 0);
-            if (SPLIT) *(uint4 *)(lo + i * 2048) = make_uint4(0, 0, 0, 0);
-          }
+        // the pair of warps loads its 32 rows, 16 each
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+          const int lr = (warp & 3) * 32 + half * 16 + i * 8 + (lane & 7), r2 = en.r0 + q * 128 + lr;
+          const int j2 = r2 / g.group, h2 = pc.head * g.group + r2 - j2 * g.group;
+          unsigned char *hi = qs + q * C::kTerms * C::kQ + lr * 16;
+          load_queries<D, T>(r2 < en.r1 ? (const T *)p.q + (en.row0 + j2) * p.q_row + h2 * p.q_head : nullptr, vec_q,
+                             p.scale, hi, hi + C::kQ, &sh.top[1][q][0][lr]);
         }
+        pair_sync(pair);
+        const float qf = sh.top[1][q][0][row];
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[q]);
         // positions of the row tile's first and last row
         const int p_lo = en.first + (en.r0 + q * 128) / g.group;
         const int p_hi = en.first + (min(en.r1, en.r0 + q * 128 + 128) - 1) / g.group;
-        for (int x = 0; x < nt && ok; x++, ns++) {
-          if (!warp_wait(&sh.s_full[q], (uint32_t)ns & 1u)) { ok = false; break; }
+        for (int x = 0; x < nt; x++, ns++) {
+          if (ok && !warp_wait(&sh.s_full[q], (uint32_t)ns & 1u)) ok = false;
           tc_fence_after();
           const int slot = (nk + x) & 3;
           const uint32_t live = sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
           const int t0 = en.tile(pc.t0 + x) * kTileKeys;
           const bool all = live == 0xffu && t0 + kTileKeys - 1 <= p_lo &&
                            (p.window <= 0 || t0 > p_hi - p.window || t0 + kTileKeys - 1 < p.sinks);
-          // Hides what the row does not see of columns c .. c + 31.
-          auto hide = [&](uint32_t (&s)[32], int c0) {
-            const int d = pos - t0 - c0 + 1;
-            uint32_t see = below(d);
-            if (p.window > 0) see &= ~below(d - p.window) | below(p.sinks - t0 - c0);
-            const uint32_t lv = live >> (c0 >> 4);
-            see &= (lv & 1u ? 0xffffu : 0u) | (lv & 2u ? 0xffff0000u : 0u);
+          if (!all) {  // -inf over what the row does not see, in tensor memory
+#pragma unroll 1
+            for (int i = 0; i < 2; i++) {
+              const int c0 = half * 64 + 32 * i, d = pos - t0 - c0 + 1;
+              uint32_t see = below(d);
+              if (p.window > 0) see &= ~below(d - p.window) | below(p.sinks - t0 - c0);
+              const uint32_t lv = live >> (c0 >> 4);
+              see &= (lv & 1u ? 0xffffu : 0u) | (lv & 2u ? 0xffff0000u : 0u);
+              uint32_t s[32];
+              tc_ld<32>(s_at + 32 * i, s);
+              tc_wait_ld<32>(s);
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              if (!((see >> e) & 1u)) s[e] = 0xff800000u;  // -inf
-          };
-          // The scores are read twice, 64 columns at a time: all 128 in
-          // registers cost spills, and unrolled four times as much code, more
-          // than the SM's instruction cache holds for its four roles.
+              for (int e = 0; e < 32; e++)
+                if (!((see >> e) & 1u)) s[e] = 0xff800000u;
+              tc_st32(s_at + 32 * i, s);
+            }
+            tc_wait_st();
+          }
+          // The scores are read twice, 32 columns at a time, in loops: the
+          // code of the four roles has to stay inside the instruction cache.
           float top = -INFINITY;
 #pragma unroll 1
-          for (int i = 0; i < 4; i += 2) {
-            uint32_t s[2][32];
-            tc_ld<32>(s_at + 32 * i, s[0]);
-            tc_ld<32>(s_at + 32 * i + 32, s[1]);
-            tc_wait_ld<32>(s[0]);
-            tc_wait_ld<32>(s[1]);
-            if (!all) {
-              hide(s[0], 32 * i);
-              hide(s[1], 32 * i + 32);
-            }
+          for (int i = 0; i < 2; i++) {
+            uint32_t s[32];
+            tc_ld<32>(s_at + 32 * i, s);
+            const int gr = half * 4 + 2 * i;
+            const float f0 = fmaxf(sh.kf[slot][gr] * qf, kTinyFactor), f1 = fmaxf(sh.kf[slot][gr + 1] * qf, kTinyFactor);
+            const float v0 = sh.lv[slot][gr], v1 = sh.lv[slot][gr + 1];
+            tc_wait_ld<32>(s);
+            float a = __uint_as_float(s[0]), b = __uint_as_float(s[16]);
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
-              float t = __uint_as_float(s[h / 2][(h & 1) * 16]);
-#pragma unroll
-              for (int e = 1; e < 16; e++) t = fmaxf(t, __uint_as_float(s[h / 2][(h & 1) * 16 + e]));
-              top = fmaxf(top, t * fmaxf(sh.kf[slot][2 * i + h] * qf, kTinyFactor) + sh.lv[slot][2 * i + h]);
+            for (int e = 1; e < 16; e++) {
+              a = fmaxf(a, __uint_as_float(s[e]));
+              b = fmaxf(b, __uint_as_float(s[16 + e]));
             }
+            top = fmaxf(top, fmaxf(a * f0 + v0, b * f1 + v1));
           }
+          sh.top[x & 1][q][half][row] = top;
+          pair_sync(pair);
+          top = fmaxf(top, sh.top[x & 1][q][half ^ 1][row]);
           const bool grow = top > m + (x ? kTileSlack : 0.0f);
           if (__any_sync(0xffffffffu, grow)) {
             const float now = grow ? top : m;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             l *= f;
             if (x) {  // every product into O before this tile's has completed (see the MMA warp)
 #pragma unroll 1
-              for (int i = 0; i < D / 32; i++) {
+              for (int i = half * (D / 64); i < (half + 1) * (D / 64); i++) {
                 uint32_t o[32];
                 tc_ld<32>(o_at + 32 * i, o);
                 tc_wait_ld<32>(o);
@@ -358,46 +358,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const uint64_t nm2 = pack2(nm, nm);
           uint64_t l2 = 0;
 #pragma unroll 1
-          for (int i = 0; i < 4; i += 2) {
-            uint32_t s[2][32];
-            tc_ld<32>(s_at + 32 * i, s[0]);
-            tc_ld<32>(s_at + 32 * i + 32, s[1]);
-            tc_wait_ld<32>(s[0]);
-            tc_wait_ld<32>(s[1]);
-            if (!all) {
-              hide(s[0], 32 * i);
-              hide(s[1], 32 * i + 32);
+          for (int i = 0; i < 2; i++) {
+            uint32_t s[32];
+            tc_ld<32>(s_at + 32 * i, s);
+            const int gr = half * 4 + 2 * i;
+            float f[2], wf[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              f[h] = fmaxf(sh.kf[slot][gr + h] * qf, kTinyFactor);
+              wf[h] = sh.wf[slot][gr + h];
             }
+            tc_wait_ld<32>(s);
+            // 32 keys: 16 columns of packed weights (and 16 of their low
+            // terms) over the scores just read
+            uint32_t w[32];
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-              // 32 keys: 16 columns of packed weights (and 16 of their low
-              // terms) over the scores just read
-              uint32_t w[32];
-#pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const int gr = 2 * (i + u) + h;
-                const float f = fmaxf(sh.kf[slot][gr] * qf, kTinyFactor), wf = sh.wf[slot][gr];
-                const uint64_t f2 = pack2(f, f), w2 = pack2(wf, wf);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                  const int at = h * 16 + 2 * e;
-                  const uint64_t a = ffma2((uint64_t)s[u][at] | ((uint64_t)s[u][at + 1] << 32), f2, nm2);
-                  const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
-                  l2 = fadd2(l2, b);
-                  const uint64_t v = fmul2(b, w2);
-                  const uint32_t pk = pack_h2(lo_of(v), hi_of(v));
-                  w[h * 8 + e] = pk;
-                  if (SPLIT) {
-                    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&pk));
-                    w[16 + h * 8 + e] = pack_h2(lo_of(v) - y.x, hi_of(v) - y.y);
-                  }
-                }
+            for (int e = 0; e < 16; e++) {
+              const int h = e / 8;
+              const uint64_t a = ffma2((uint64_t)s[2 * e] | ((uint64_t)s[2 * e + 1] << 32), pack2(f[h], f[h]), nm2);
+              const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
+              l2 = fadd2(l2, b);
+              const uint64_t v = fmul2(b, pack2(wf[h], wf[h]));
+              w[e] = pack_h2(lo_of(v), hi_of(v));
+              if (SPLIT) {
+                const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+                w[16 + e] = pack_h2(lo_of(v) - y.x, hi_of(v) - y.y);
               }
-              if constexpr (SPLIT) {
-                tc_st32(s_at + 32 * (i + u), w);
-              } else {
-                tc_st16(s_at + 32 * (i + u), w);
-              }
+            }
+            if constexpr (SPLIT) {
+              tc_st32(s_at + 32 * i, w);
+            } else {
+              tc_st16(s_at + 32 * i, w);
             }
           }
           l += lo_of(l2) + hi_of(l2);
@@ -406,52 +397,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.p_full[q]);
         }
+        // the row's sum from both halves
+        sh.top[nt & 1][q][half][row] = l;
+        pair_sync(pair);
+        l += sh.top[nt & 1][q][half ^ 1][row];
+        pair_sync(pair);  // read before the next piece's queries write there
       }
       nk += nt;
       // ---- the piece's result ----
       const int kPart = kTileRows * (D + 2);
       float *part = g.parts + (int64_t)(pc.starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x) * kPart;
-      if (on && ok) {
+      if (on) {
         if (nt > 0) {
-          if (!warp_wait(&sh.pv_done[q], (uint32_t)(ns - 1) & 1u)) ok = false;
+          if (ok && !warp_wait(&sh.pv_done[q], (uint32_t)(ns - 1) & 1u)) ok = false;
           tc_fence_after();
         }
         const int pr = q * 128 + row;  // row of the item
         const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / (l * kTileShift)) : 1.0f;
         T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
 #pragma unroll 1
-        for (int hf = 0; hf < D / 64; hf++) {
-          uint32_t o[2][32];
+        for (int i = half * (D / 64); i < (half + 1) * (D / 64); i++) {
+          uint32_t o[32];
           if (nt > 0) {
-            tc_ld<32>(o_at + 64 * hf, o[0]);
-            tc_ld<32>(o_at + 64 * hf + 32, o[1]);
-            tc_wait_ld<32>(o[0]);
-            tc_wait_ld<32>(o[1]);
+            tc_ld<32>(o_at + 32 * i, o);
+            tc_wait_ld<32>(o);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e++) o[0][e] = o[1][e] = 0;
+            for (int e = 0; e < 32; e++) o[e] = 0;
           }
           if (mine) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) {  // elements 16 t .. 16 t + 15 of this half
-              float v[16];
+            for (int t = 0; t < 4; t++) {  // 8 consecutive elements
+              float v[8];
 #pragma unroll
-              for (int e = 0; e < 16; e++) {
-                const int n = 8 * (e / 2) + 2 * t + (e & 1);
-                v[e] = __uint_as_float(o[n / 32][n % 32]) * inv;
-              }
-              const int d0 = hf * 64 + t * 16;
+              for (int e = 0; e < 8; e++) v[e] = __uint_as_float(o[8 * (e / 2) + 2 * t + (e & 1)]) * inv;
+              const int d0 = (i >> 1) * 64 + t * 16 + (i & 1) * 8;
               if (!pc.whole) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                  *(float4 *)(part + (int64_t)pr * D + d0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                *(float4 *)(part + (int64_t)pr * D + d0) = make_float4(v[0], v[1], v[2], v[3]);
+                *(float4 *)(part + (int64_t)pr * D + d0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
               } else {
-                store16<T>(dst + d0, v, vec_o);
+                store_row<T, 8>(dst + d0, v, vec_o);
               }
             }
           }
         }
-        if (mine) {
+        if (mine && half == 0) {
           if (pc.whole) {
             if (p.lse) p.lse[(en.row0 + j) * p.n_heads + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
           } else {
@@ -474,7 +464,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (sh.last) {
           __threadfence();
           // a thread joins 16 elements of a row
-          for (int u = tid; u < nr * (D / 16); u += 256) {
+          for (int u = tid; u < nr * (D / 16); u += 512) {
             const int rr = u / (D / 16), d0 = u % (D / 16) * 16;
             float top = -INFINITY, sum = 0.0f, acc[16];
             for (int k = 0; k < pc.parts; k++)
@@ -501,7 +491,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[e] *= inv;
-            store16<T>(dst, acc, vec_o);
+            store_row<T, 16>(dst, acc, vec_o);
             if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
           }
@@ -509,9 +499,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         soft_sync();  // sh.last is free
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ================= converters =================
-    const int w = warp - 8;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    const int w = warp - 16;
     constexpr int HF = D / 64;
     const int nblk = c.page / c.block;
     int nk = 0;
@@ -644,64 +635,77 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else {
     // ================= MMA =================
-    if (lane == 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 20) {
+      // the whole warp walks the tiles (so that addresses stay in uniform
+      // registers), one lane issues
+      const bool lead = elect_one();
       const uint32_t id_s = umma_idesc_f16(128), id_o = umma_idesc_f16(D);
       const uint64_t q0 = umma_desc(qs, 2048, 128), k0 = umma_desc(kt, 2048, 128), v0 = umma_desc(vt, D * 16, 128);
-      int nq[2] = {0, 0}, ns[2] = {0, 0}, np[2] = {0, 0}, nk = 0;
-      // S of row tile q from key tile stage st: when the last product that
-      // read its weights (they lie over the scores) has completed
-      auto scores = [&](int q, int st) {
-        if (np[q] > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np[q] - 1) & 1u)) return false;
+      int np0 = 0, np1 = 0, nq0 = 0, nq1 = 0, nk = 0;  // products into O, pieces of each row tile, key tiles
+      // S of row tile q from K stage st, once the last product that read its
+      // weights (they lie over the scores) has completed
+      auto scores = [&](int q, int np, int st, bool last) {
+        if (np > 0 && !warp_wait(&sh.pv_done[q], (uint32_t)(np - 1) & 1u)) return false;
         tc_fence_after();
+        if (lead) {
+          const uint64_t kd = k0 + (uint64_t)((st * C::kKv) >> 4);
 #pragma unroll
-        for (int t = 0; t < C::kTerms; t++)
+          for (int t = 0; t < C::kTerms; t++)  // low terms first: less of them is lost to the large sums
 #pragma unroll
-          for (int i = 0; i < D / 16; i++)
-            tc_mma_f16(tmem + q * 128,
-                       q0 + (uint64_t)(((q * C::kTerms + C::kTerms - 1 - t) * C::kQ + i * 4096) >> 4),
-                       k0 + (uint64_t)((st * C::kKv + i * 4096) >> 4), id_s, (uint32_t)(t | i));
-        mbar_arrive(&sh.s_full[q]);
-        tc_commit(&sh.s_full[q]);
-        ns[q]++;
+            for (int i = 0; i < D / 16; i++)
+              tc_mma_f16(tmem + q * 128, q0 + (uint64_t)(((q * C::kTerms + C::kTerms - 1 - t) * C::kQ + i * 4096) >> 4),
+                         kd + (uint64_t)((i * 4096) >> 4), id_s, (uint32_t)(t | i));
+          mbar_arrive(&sh.s_full[q]);
+          tc_commit(&sh.s_full[q]);
+          if (last) tc_commit(&sh.k_empty[st]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto output = [&](int q, int np, int st, bool first, bool last) {
+        if (!warp_wait(&sh.p_full[q], (uint32_t)np & 1u)) return false;
+        tc_fence_after();
+        if (lead) {
+          const uint64_t vd = v0 + (uint64_t)((st * C::kKv) >> 4);
+#pragma unroll
+          for (int t = 0; t < C::kTerms; t++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + (i >> 1) * 32 + t * 16 + (i & 1) * 8,
+                        vd + (uint64_t)((i * 2 * D * 16) >> 4), id_o, t | i ? 1u : first ? 0u : 1u);
+          tc_commit(&sh.pv_done[q]);
+          if (last) tc_commit(&sh.v_empty[st]);
+        }
+        __syncwarp();
         return true;
       };
       while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
         const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
         if (nt == 0) continue;
-        const int tiles = en.r1 - en.r0 > 128 ? 2 : 1;
-        for (int x = -1; x < nt && ok; x++) {
-          // after O += W V of tile x (row tile q): S of tile x + 1
+        const bool two = en.r1 - en.r0 > 128;
+        ok = warp_wait(&sh.q_full[0], (uint32_t)nq0++ & 1u) && warp_wait(&sh.k_full[nk % NS], (uint32_t)(nk / NS) & 1u) &&
+             scores(0, np0, nk % NS, !two);
+        if (ok && two) ok = warp_wait(&sh.q_full[1], (uint32_t)nq1++ & 1u) && scores(1, np1, nk % NS, true);
+        for (int x = 0; x < nt && ok; x++) {
+          // O += W V of tile x, then S of tile x + 1: first one row tile, then the other
           const int st = (nk + x) % NS, st1 = (nk + x + 1) % NS;
-          for (int q = 0; q < tiles && ok; q++) {
-            if (x >= 0) {
-              if (q == 0 && !mbar_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u)) { ok = false; break; }
-              if (!mbar_wait(&sh.p_full[q], (uint32_t)np[q] & 1u)) { ok = false; break; }
-              tc_fence_after();
-#pragma unroll
-              for (int t = 0; t < C::kTerms; t++)
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                  tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + (i >> 1) * 32 + t * 16 + (i & 1) * 8,
-                            v0 + (uint64_t)((st * C::kKv + i * 2 * D * 16) >> 4), id_o, (uint32_t)(x | t | i));
-              tc_commit(&sh.pv_done[q]);
-              np[q]++;
-              if (q == tiles - 1) tc_commit(&sh.v_empty[st]);
-            } else {
-              if (!mbar_wait(&sh.q_full[q], (uint32_t)nq[q] & 1u)) { ok = false; break; }
-              nq[q]++;
-            }
-            if (x + 1 < nt) {
-              if (q == 0 && !mbar_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u)) { ok = false; break; }
-              if (!scores(q, st1)) { ok = false; break; }
-              if (q == tiles - 1) tc_commit(&sh.k_empty[st1]);
-            }
+          const bool more = x + 1 < nt;
+          ok = warp_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u) && output(0, np0, st, x == 0, !two);
+          np0++;
+          if (ok && more)
+            ok = warp_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u) && scores(0, np0, st1, !two);
+          if (ok && two) {
+            ok = output(1, np1, st, x == 0, true);
+            np1++;
+            if (ok && more) ok = scores(1, np1, st1, true);
           }
         }
         nk += nt;
       }
       // every product completes before the tensor memory is released
-      for (int q = 0; q < 2; q++)
-        if (np[q] > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np[q] - 1) & 1u)) ok = false;
+      if (np0 > 0 && !warp_wait(&sh.pv_done[0], (uint32_t)(np0 - 1) & 1u)) ok = false;
+      if (np1 > 0 && !warp_wait(&sh.pv_done[1], (uint32_t)(np1 - 1) & 1u)) ok = false;
     }
     __syncwarp();
   }
@@ -709,7 +713,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12)
+  if (warp == 20)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
