@@ -37,7 +37,8 @@ struct Layer {
   uint32_t *status;
   int n_pages, n_seqs, max_pages;
   int kv, page, block;
-  int page_shift;  // log2(page), or -1
+  int block_shift;      // log2(block)
+  uint32_t page_magic;  // 2^32 / (page / 16), rounded up; 0 for a page of 16
 };
 
 // The rows of a call: row r of sequence i (of m) is packed row start(i) + r
@@ -77,8 +78,17 @@ __device__ __forceinline__ int seq_length(const Layer &c, int s) {
   return n < 0 ? 0 : (int64_t)n > most ? (int)most : n;
 }
 
+// Page index of a token: n / d with n = token / 16 < 2^26 and d = page / 16
+// <= 64 by a product with 2^32 / d rounded up, which is off by less than
+// n / 2^32 < 1 / 64: exact, as n / d has no fraction above 1 - 1 / d.
 __device__ __forceinline__ int page_of(const Layer &c, int tok) {
-  return c.page_shift >= 0 ? tok >> c.page_shift : (int)((unsigned)tok / (unsigned)c.page);
+  const uint32_t n = (uint32_t)tok >> 4;
+  return c.page_magic ? (int)__umulhi(n, c.page_magic) : (int)n;
+}
+
+// Starts moving bytes (a multiple of 16, 16-byte aligned) to the L2 cache.
+__device__ __forceinline__ void prefetch_l2(const void *p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 template <typename T>

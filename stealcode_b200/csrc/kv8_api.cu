@@ -81,9 +81,9 @@ kv8::Layer layer_of(const sc_kv8_cache *c, int64_t layer) {
   l.kv = c->n_kv_heads;
   l.page = c->page;
   l.block = c->block;
-  l.page_shift = -1;
-  for (int s = 4; s <= 10; s++)
-    if (c->page == 1 << s) l.page_shift = s;
+  l.block_shift = c->block == 16 ? 4 : c->block == 32 ? 5 : 6;
+  const uint32_t d = (uint32_t)c->page / 16;
+  l.page_magic = d == 1 ? 0 : (uint32_t)(((1ull << 32) + d - 1) / d);
   return l;
 }
 

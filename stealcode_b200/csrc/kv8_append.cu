@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
   const int h = blockIdx.y, z = blockIdx.z;
   const T *src = (const T *)(z ? p.v : p.k) + (int64_t)h * (z ? p.v_head : p.k_head);
   const int64_t ld = z ? p.v_row : p.k_row;
-  const int slot0 = b0 % c.page;
+  const int slot0 = b0 - page_of(c, b0) * c.page;
   const int64_t ph = (int64_t)pid * c.kv + h;
   int8_t *dst = (z ? c.v : c.k) + (ph * c.page + slot0) * D;
   float *sp = (z ? c.vs : c.ks) + ph * (c.page / c.block) + slot0 / c.block;
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   const int tok = s < 0 ? -1 : seq_length(c, s) - count + j;
   const int pid = tok < 0 ? -1 : c.table[(int64_t)s * c.max_pages + page_of(c, tok)];
   const bool ok = (unsigned)pid < (unsigned)c.n_pages;
-  const int h = blockIdx.y, slot = tok < 0 ? 0 : tok % c.page;
+  const int h = blockIdx.y, slot = tok < 0 ? 0 : tok - page_of(c, tok) * c.page;
   const int64_t ph = (int64_t)(ok ? pid : 0) * c.kv + h;
   constexpr int E = D / 32;
 #pragma unroll

@@ -80,9 +80,10 @@ struct StepShared {
 
 // The 16 tokens of a warp in one tile.
 struct Group {
-  int tok;          // first token
-  bool live;        // some row sees some of them, and they have a page
-  int64_t at, sat;  // token's offset in units of rows (of D codes), scale's offset
+  int tok;      // first token
+  bool live;    // some row sees some of them, and they have a page
+  int64_t at;   // offset of the first token's codes, from the head's first
+  int64_t sat;  // of its scale
 };
 
 template <int D, int NT, typename T>
@@ -96,15 +97,80 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
   extern __shared__ __align__(16) unsigned char smem[];
   S &sh = *reinterpret_cast<S *>(smem);
   const Layer &c = p.c;
-  const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
+  const int tid = (int)threadIdx.x, lane = tid & 31, gi = lane >> 2, ti = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same in all lanes: addresses stay in uniform registers
 
   Share share;
   if (!find_share<ROWS, kStepTile, kStepOver, kStepThreads>(p, g, sh.share, share)) return;
   Entry en;
   Piece pc;
   const int nblk = c.page / c.block;
+  const int page_bytes = c.kv * c.page * D, page_scales = c.kv * nblk;  // of one page, K or V
   while (next_piece<ROWS, kStepTile, kStepOver>(p, g, share, en, pc)) {
     const int nr = en.r1 - en.r0;
+    // ---- the keys' and values' first loads ----
+    const int t1 = min(pc.t1, en.tiles());
+    const int32_t *trow = c.table + (int64_t)max(en.s, 0) * c.max_pages;
+    const int8_t *kh = c.k + (int64_t)pc.head * c.page * D, *vh = c.v + (int64_t)pc.head * c.page * D;
+    const float *ksh = c.ks + pc.head * nblk, *vsh = c.vs + pc.head * nblk;
+    auto token = [&](int x) { return x < t1 ? en.tile(x) * kStepTile + warp * 16 : -1; };
+    auto page_id = [&](int tok) {
+      const bool in = tok >= 0 && tok <= en.p_hi &&
+                      (p.window <= 0 || tok + 15 > en.p_lo - p.window || tok < p.sinks);
+      return in ? trow[page_of(c, tok)] : -1;
+    };
+    auto group = [&](int tok, int pid) {
+      Group q;
+      q.tok = tok;
+      q.live = (unsigned)pid < (unsigned)c.n_pages;
+      if (!q.live && pid >= 0 && lane == 0) atomicOr(c.status, kBadPage);
+      const int slot = tok - page_of(c, tok) * c.page;
+      q.at = (int64_t)pid * page_bytes + slot * D;
+      q.sat = (int64_t)pid * page_scales + (slot >> c.block_shift);
+      return q;
+    };
+    uint4 kr[2][HF];
+    uint32_t vr[4][D / 32];
+    float ks = 0.0f, vs = 0.0f;
+    auto load_k = [&](const Group &q) {
+      if (!q.live) return;
+      const int8_t *src = kh + q.at + (gi * D + ti * 16);
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int f = 0; f < HF; f++) kr[u][f] = __ldg((const uint4 *)(src + 8 * u * D + f * 64));
+      ks = __ldg(ksh + q.sat);
+      vs = __ldg(vsh + q.sat);
+    };
+    auto load_v = [&](const Group &q) {
+      if (!q.live) return;
+      const int8_t *base = vh + q.at + (2 * ti * D + gi * (D / 8));
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int8_t *src = base + ((u & 1) + (u >> 1) * 8) * D;
+        if constexpr (D == 128) {
+          const uint4 x = __ldg((const uint4 *)src);
+          vr[u][0] = x.x; vr[u][1] = x.y; vr[u][2] = x.z; vr[u][3] = x.w;
+        } else {
+          const uint2 x = __ldg((const uint2 *)src);
+          vr[u][0] = x.x; vr[u][1] = x.y;
+        }
+      }
+    };
+    // A group's codes are on their way to L2 one step before its loads into
+    // registers: HBM's latency is longer than one step of a warp hides.
+    auto ahead = [&](const Group &q) {
+      if (q.live && lane < 2) prefetch_l2((lane ? vh : kh) + q.at, 16 * D);
+    };
+    int tok2 = token(pc.t0 + 1);
+    Group cur = group(token(pc.t0), page_id(token(pc.t0)));
+    int pid2 = page_id(tok2);
+    load_k(cur);
+    load_v(cur);
+    Group nxt = group(tok2, pid2);
+    ahead(nxt);
+    tok2 = token(pc.t0 + 2);
+    pid2 = page_id(tok2);
     // ---- the rows of q: one warp a row ----
     for (int r = warp; r < ROWS; r += 4) {
       float v[D / 32];
@@ -164,68 +230,16 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       l[n][0] = l[n][1] = 0.0f;
     }
 
-    const int t1 = min(pc.t1, en.tiles());
-    const int32_t *trow = c.table + (int64_t)max(en.s, 0) * c.max_pages;
-    auto token = [&](int x) { return x < t1 ? en.tile(x) * kStepTile + warp * 16 : -1; };
-    auto page_id = [&](int tok) {
-      const bool in = tok >= 0 && tok <= en.p_hi &&
-                      (p.window <= 0 || tok + 15 > en.p_lo - p.window || tok < p.sinks);
-      return in ? trow[page_of(c, tok)] : -1;
-    };
-    auto group = [&](int tok, int pid) {
-      Group q;
-      q.tok = tok;
-      q.live = (unsigned)pid < (unsigned)c.n_pages;
-      if (!q.live && pid >= 0 && lane == 0) atomicOr(c.status, kBadPage);
-      const int slot = tok - page_of(c, tok) * c.page;
-      const int64_t ph = (int64_t)pid * c.kv + pc.head;
-      q.at = ph * c.page + slot;
-      q.sat = ph * nblk + slot / c.block;
-      return q;
-    };
-    uint4 kr[2][HF];
-    uint32_t vr[4][D / 32];
-    float ks = 0.0f, vs = 0.0f;
-    auto load_k = [&](const Group &q) {
-      if (!q.live) return;
-      const int8_t *src = c.k + q.at * D + ti * 16;
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int f = 0; f < HF; f++)
-          kr[u][f] = __ldg((const uint4 *)(src + (gi + 8 * u) * D + f * 64));
-      ks = __ldg(c.ks + q.sat);
-      vs = __ldg(c.vs + q.sat);
-    };
-    auto load_v = [&](const Group &q) {
-      if (!q.live) return;
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const int8_t *src = c.v + (q.at + 2 * ti + (u & 1) + (u >> 1) * 8) * D + gi * (D / 8);
-        if constexpr (D == 128) {
-          const uint4 x = __ldg((const uint4 *)src);
-          vr[u][0] = x.x; vr[u][1] = x.y; vr[u][2] = x.z; vr[u][3] = x.w;
-        } else {
-          const uint2 x = __ldg((const uint2 *)src);
-          vr[u][0] = x.x; vr[u][1] = x.y;
-        }
-      }
-    };
-
-    int tok_n = token(pc.t0), pid_n = page_id(tok_n);
-    Group cur = group(tok_n, pid_n);
-    load_k(cur);
-    load_v(cur);
-    tok_n = token(pc.t0 + 1);
-    pid_n = page_id(tok_n);
     for (int x = pc.t0; x < t1; x++) {
-      const Group nxt = group(tok_n, pid_n);
-      tok_n = token(x + 2);
-      pid_n = page_id(tok_n);
+      const Group nxt2 = group(tok2, pid2);
+      ahead(nxt2);
+      tok2 = token(x + 3);
+      pid2 = page_id(tok2);
       if (!cur.live) {
         load_k(nxt);
         load_v(nxt);
         cur = nxt;
+        nxt = nxt2;
         continue;
       }
       // ---- S^T = K Q^T ----
@@ -333,6 +347,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       }
       load_v(nxt);
       cur = nxt;
+      nxt = nxt2;
     }
 
     // ---- join the four warps ----

@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t s_at = tmem + lanes + (uint32_t)(q * 128 + half * 64), o_at = tmem + lanes + (uint32_t)(256 + q * 128);
     int ns = 0;   // tiles this row tile has gone through
     int nk = 0;   // key tiles of the block (slots of the scale ring)
-    // a wait that gave up (ok false) ends the products, not the loop: every
-    // warp reaches the same barriers
+    // a wait that gave up (ok false) is the last one of its thread; the loops
+    // run to their end, so every warp reaches the same barriers
     while (next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
       const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
       const int nr = en.r1 - en.r0;
@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int p_lo = en.first + (en.r0 + q * 128) / g.group;
         const int p_hi = en.first + (min(en.r1, en.r0 + q * 128 + 128) - 1) / g.group;
         for (int x = 0; x < nt; x++, ns++) {
-          if (ok && !warp_wait(&sh.s_full[q], (uint32_t)ns & 1u)) ok = false;
+          if (ok) ok = mbar_wait(&sh.s_full[q], (uint32_t)ns & 1u);
+          __syncwarp();
           tc_fence_after();
           const int slot = (nk + x) & 3;
           const uint32_t live = sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float *part = g.parts + (int64_t)(pc.starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x) * kPart;
       if (on) {
         if (nt > 0) {
-          if (ok && !warp_wait(&sh.pv_done[q], (uint32_t)(ns - 1) & 1u)) ok = false;
+          if (ok) ok = mbar_wait(&sh.pv_done[q], (uint32_t)(ns - 1) & 1u);
+          __syncwarp();
           tc_fence_after();
         }
         const int pr = q * 128 + row;  // row of the item
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int HF = D / 64;
     const int nblk = c.page / c.block;
     int nk = 0;
-    while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
+    while (next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
       const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
       if (nt == 0) continue;
       const int32_t *trow = c.table + (int64_t)en.s * c.max_pages;
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (id >= 0) {
             const int tok = en.tile(pc.t0 + x) * kTileKeys + w * 32 + lane * 16;
             const int slot = tok - page_of(c, tok) * c.page;
-            const int64_t at = ((int64_t)id * c.kv + pc.head) * nblk + slot / c.block;
+            const int64_t at = ((int64_t)id * c.kv + pc.head) * nblk + (slot >> c.block_shift);
             ks = __ldg(c.ks + at);
             vs = __ldg(c.vs + at);
           }
@@ -575,7 +577,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int x = 0; x < nt; x++, nk++) {
         const int st = nk % NS;
         const uint32_t turn = (uint32_t)(nk / NS) & 1u;
-        if (!warp_wait(&sh.k_empty[st], turn ^ 1u)) { ok = false; break; }
+        if (ok) ok = mbar_wait(&sh.k_empty[st], turn ^ 1u);
+        __syncwarp();
         unsigned char *kd = kt + st * C::kKv;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -605,7 +608,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[st]);
         if (x + 1 < nt) load_k(x + 1, nxt);
-        if (!warp_wait(&sh.v_empty[st], turn ^ 1u)) { ok = false; break; }
+        if (ok) ok = mbar_wait(&sh.v_empty[st], turn ^ 1u);
+        __syncwarp();
         const uint32_t vd = smem_u32(vt + st * C::kKv);
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -646,7 +650,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // S of row tile q from K stage st, once the last product that read its
       // weights (they lie over the scores) has completed
       auto scores = [&](int q, int np, int st, bool last) {
-        if (np > 0 && !warp_wait(&sh.pv_done[q], (uint32_t)(np - 1) & 1u)) return false;
+        if (np > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np - 1) & 1u)) return false;
         tc_fence_after();
         if (lead) {
           const uint64_t kd = k0 + (uint64_t)((st * C::kKv) >> 4);
@@ -660,11 +664,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_commit(&sh.s_full[q]);
           if (last) tc_commit(&sh.k_empty[st]);
         }
-        __syncwarp();
         return true;
       };
       auto output = [&](int q, int np, int st, bool first, bool last) {
-        if (!warp_wait(&sh.p_full[q], (uint32_t)np & 1u)) return false;
+        if (!mbar_wait(&sh.p_full[q], (uint32_t)np & 1u)) return false;
         tc_fence_after();
         if (lead) {
           const uint64_t vd = v0 + (uint64_t)((st * C::kKv) >> 4);
@@ -677,39 +680,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_commit(&sh.pv_done[q]);
           if (last) tc_commit(&sh.v_empty[st]);
         }
-        __syncwarp();
         return true;
       };
       while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
         const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
         if (nt == 0) continue;
         const bool two = en.r1 - en.r0 > 128;
-        ok = warp_wait(&sh.q_full[0], (uint32_t)nq0++ & 1u) && warp_wait(&sh.k_full[nk % NS], (uint32_t)(nk / NS) & 1u) &&
+        ok = mbar_wait(&sh.q_full[0], (uint32_t)nq0++ & 1u) && mbar_wait(&sh.k_full[nk % NS], (uint32_t)(nk / NS) & 1u) &&
              scores(0, np0, nk % NS, !two);
-        if (ok && two) ok = warp_wait(&sh.q_full[1], (uint32_t)nq1++ & 1u) && scores(1, np1, nk % NS, true);
+        if (ok && two) ok = mbar_wait(&sh.q_full[1], (uint32_t)nq1++ & 1u) && scores(1, np1, nk % NS, true);
+        ok = __all_sync(0xffffffffu, ok);  // lanes poll by themselves; one that gave up ends the loop for all
         for (int x = 0; x < nt && ok; x++) {
           // O += W V of tile x, then S of tile x + 1: first one row tile, then the other
           const int st = (nk + x) % NS, st1 = (nk + x + 1) % NS;
           const bool more = x + 1 < nt;
-          ok = warp_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u) && output(0, np0, st, x == 0, !two);
+          ok = mbar_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u) && output(0, np0, st, x == 0, !two);
           np0++;
           if (ok && more)
-            ok = warp_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u) && scores(0, np0, st1, !two);
+            ok = mbar_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u) && scores(0, np0, st1, !two);
           if (ok && two) {
             ok = output(1, np1, st, x == 0, true);
             np1++;
             if (ok && more) ok = scores(1, np1, st1, true);
           }
+          ok = __all_sync(0xffffffffu, ok);
         }
         nk += nt;
       }
       // every product completes before the tensor memory is released
-      if (np0 > 0 && !warp_wait(&sh.pv_done[0], (uint32_t)(np0 - 1) & 1u)) ok = false;
-      if (np1 > 0 && !warp_wait(&sh.pv_done[1], (uint32_t)(np1 - 1) & 1u)) ok = false;
+      if (np0 > 0 && !mbar_wait(&sh.pv_done[0], (uint32_t)(np0 - 1) & 1u)) ok = false;
+      if (np1 > 0 && !mbar_wait(&sh.pv_done[1], (uint32_t)(np1 - 1) & 1u)) ok = false;
     }
     __syncwarp();
   }
-  if (!ok && lane == 0) atomicOr(c.status, kWaitTimeout);
+  if (!ok) atomicOr(c.status, kWaitTimeout);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -22,7 +22,6 @@ the host; failures that only the device sees (too few free pages) are read with
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from ctypes import c_int32, c_int64, c_void_p
 
@@ -41,6 +40,12 @@ _FAILURES = (
     (BAD_PAGE, SC_ERR_INVALID, "a page id outside the cache, or an append without a reserved page"),
     (WAIT_TIMEOUT, SC_ERR_TIMEOUT, "a bounded device-side wait gave up"),
 )
+
+
+# The current stream's handle without building a torch.cuda.Stream (5 us of a 10 us call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class _Cache(ctypes.Structure):
@@ -96,6 +101,7 @@ class KvCache8:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.table, self.length, self.refs = table, length, refs
         self.device = k.device
+        self._index = k.device.index
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.n_layers, self.n_pages, self.n_kv_heads, self.page, self.head_dim = k.shape
         self.block = self.page // k_scale.shape[3]
@@ -109,14 +115,16 @@ class KvCache8:
     # ---- arguments ----------------------------------------------------------------
 
     def _stream(self, stream) -> int:
-        if torch.cuda.current_device() != self.device.index:
-            raise ValueError(f"the cache lives on {self.device}, the current device is {torch.cuda.current_device()}")
-        return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+        if _current_device() != self._index:
+            raise ValueError(f"the cache lives on {self.device}, the current device is {_current_device()}")
+        return _raw_stream(self._index) if stream is None else stream.cuda_stream
 
-    @staticmethod
-    def _on(stream):
-        """Allocations belong to the stream that uses them."""
-        return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+    def _empty(self, stream, *args, **kw):
+        """torch.empty on the stream that will use it."""
+        if stream is None:
+            return torch.empty(*args, device=self.device, **kw)
+        with torch.cuda.stream(stream):
+            return torch.empty(*args, device=self.device, **kw)
 
     def _ids(self, t, name: str) -> int:
         if t is None:
@@ -125,12 +133,15 @@ class KvCache8:
             raise ValueError(f"{name} has to be a contiguous int32 tensor [m] on {self.device}")
         return t.data_ptr()
 
-    def _workspace(self, kind: str, stream: int, need) -> torch.Tensor:
-        ws = self._ws.get((kind, stream))
+    def _workspace(self, kind: str, st: int, stream, need) -> tuple:
+        """(address, bytes) of this stream's workspace, zeroed when it is made."""
+        ws = self._ws.get((kind, st))
         if ws is None:
             n = need()
             check(min(n, 0))
-            ws = self._ws[(kind, stream)] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            with torch.cuda.stream(torch.cuda.current_stream() if stream is None else stream):
+                buf = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            ws = self._ws[(kind, st)] = (buf.data_ptr(), n, buf)
         return ws
 
     def _batch(self, seqs, cu, n, total):
@@ -167,8 +178,11 @@ class KvCache8:
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError("k and v differ in type or shape")
         b = self._batch(seqs, cu, n, k.shape[0])
-        check(lib.sc_kv8_append(self._p, layer, ctypes.addressof(b), k.data_ptr(), k.stride(0), k.stride(1),
-                                v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype], self._stream(stream)))
+        ks, vs = k.stride(), v.stride()
+        rc = lib.sc_kv8_append(self._p, layer, ctypes.byref(b), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                               _DTYPES[k.dtype], self._stream(stream))
+        if rc:
+            check(rc)
 
     def rows(self, layer: int, *, seqs=None, cu=None, n=None, total=None, dtype=torch.float32, stream=None):
         """The stored values (k, v), each [rows, n_kv_heads, head_dim], of the sequences' last tokens; with
@@ -177,10 +191,11 @@ class KvCache8:
         if dtype not in _DTYPES:
             raise ValueError("dtype has to be f32, f16 or bf16")
         st = self._stream(stream)
-        with self._on(stream):
-            k, v = (torch.empty(b.total, self.n_kv_heads, self.head_dim, dtype=dtype, device=self.device)
-                    for _ in range(2))
-        check(lib.sc_kv8_rows(self._p, layer, ctypes.addressof(b), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], st))
+        shape = (b.total, self.n_kv_heads, self.head_dim)
+        k, v = self._empty(stream, shape, dtype=dtype), self._empty(stream, shape, dtype=dtype)
+        rc = lib.sc_kv8_rows(self._p, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], st)
+        if rc:
+            check(rc)
         return k, v
 
     def attend(self, layer: int, q, *, seqs=None, cu=None, n=None, max_len: int = 0, window: int = 0, sinks: int = 0,
@@ -193,29 +208,31 @@ class KvCache8:
         ``max_len``: no sequence is longer (sizes the launch).  ``scale``: head_dim ** -0.5 if None."""
         if q.dim() != 3 or q.shape[1] < 1:
             raise ValueError("q has to be [rows, n_heads, head_dim]")
-        self._rows_in(q, q.shape[1], "q")
+        heads = q.shape[1]
+        self._rows_in(q, heads, "q")
         b = self._batch(seqs, cu, n, q.shape[0])
         st = self._stream(stream)
-        with self._on(stream):
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            else:
-                self._rows_in(out, q.shape[1], "out")
-                if out.dtype != q.dtype or out.shape != q.shape:
-                    raise ValueError("out has to have q's type and shape")
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
-            ws = self._workspace("attend", st, lib.sc_kv8_attend_workspace_bytes)
-        check(lib.sc_kv8_attend(self._p, layer, ctypes.addressof(b), q.data_ptr(), q.stride(0), q.stride(1),
-                                q.shape[1], self.head_dim ** -0.5 if scale is None else scale, window, sinks, max_len,
-                                out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr() if return_lse else None,
-                                _DTYPES[q.dtype], ws.data_ptr(), ws.numel(), st))
+        if out is None:
+            out = self._empty(stream, q.shape, dtype=q.dtype)
+        else:
+            self._rows_in(out, heads, "out")
+            if out.dtype != q.dtype or out.shape != q.shape:
+                raise ValueError("out has to have q's type and shape")
+        lse = self._empty(stream, q.shape[:2], dtype=torch.float32) if return_lse else None
+        ws = self._workspace("attend", st, stream, lib.sc_kv8_attend_workspace_bytes)
+        qs, os_ = q.stride(), out.stride()
+        rc = lib.sc_kv8_attend(self._p, layer, ctypes.byref(b), q.data_ptr(), qs[0], qs[1], heads,
+                               self.head_dim ** -0.5 if scale is None else scale, window, sinks, max_len,
+                               out.data_ptr(), os_[0], os_[1], lse.data_ptr() if return_lse else None,
+                               _DTYPES[q.dtype], ws[0], ws[1], st)
+        if rc:
+            check(rc)
         return (out, lse) if return_lse else out
 
     # ---- pages --------------------------------------------------------------------
 
     def _page_ws(self, st: int, stream):
-        with self._on(stream):
-            return self._workspace("pages", st, lambda: lib.sc_kv8_page_workspace_bytes(self._p))
+        return self._workspace("pages", st, stream, lambda: lib.sc_kv8_page_workspace_bytes(self._p))
 
     def reserve(self, counts, *, seqs=None, stream=None) -> None:
         """Pages for counts[i] more tokens (int32 CUDA tensor [m]) of each sequence; the lengths grow."""
@@ -224,7 +241,7 @@ class KvCache8:
             raise ValueError("seqs and counts differ in length")
         st = self._stream(stream)
         ws = self._page_ws(st, stream)
-        check(lib.sc_kv8_reserve(self._p, self._ids(seqs, "seqs"), p, counts.shape[0], ws.data_ptr(), ws.numel(), st))
+        check(lib.sc_kv8_reserve(self._p, self._ids(seqs, "seqs"), p, counts.shape[0], ws[0], ws[1], st))
 
     def fork(self, parents, children, *, stream=None) -> None:
         """children[i] becomes a copy of parents[i] (int32 CUDA tensors [m]; all pairs at once, so a parent
@@ -235,7 +252,7 @@ class KvCache8:
             raise ValueError("parents and children differ in length")
         st = self._stream(stream)
         ws = self._page_ws(st, stream)
-        check(lib.sc_kv8_fork(self._p, a, b, parents.shape[0], ws.data_ptr(), ws.numel(), st))
+        check(lib.sc_kv8_fork(self._p, a, b, parents.shape[0], ws[0], ws[1], st))
 
     def release(self, seqs=None, *, stream=None) -> None:
         """Give back the sequences' pages; their lengths become 0.  None: all sequences."""
@@ -251,7 +268,7 @@ class KvCache8:
         """Move the pages in use to the lowest ids; the tables follow."""
         st = self._stream(stream)
         ws = self._page_ws(st, stream)
-        check(lib.sc_kv8_compact(self._p, ws.data_ptr(), ws.numel(), st))
+        check(lib.sc_kv8_compact(self._p, ws[0], ws[1], st))
 
     def check(self) -> None:
         """Raise ScError if a call failed on the device (synchronises); ``clear_status`` forgets it."""
