@@ -17,6 +17,7 @@ namespace sc {
 namespace kv8 {
 
 constexpr float kTiny = 1e-30f;
+constexpr int kStepRows = 8;  // up to this many rows a sequence, a warp takes a block
 
 __device__ __forceinline__ float finite_mag(float x) {
   const float a = fabsf(x);
@@ -29,18 +30,25 @@ __device__ __forceinline__ int8_t code_of(float x, float inv) {
   return (int8_t)(int)fminf(fmaxf(r, -127.0f), 127.0f);
 }
 
-// One warp writes one touched block of one head, of K (z = 0) or V (z = 1).
+// One touched block of one head, of K (z = 0) or V (z = 1).
+template <typename T>
+struct Touched {
+  const T *src;   // the row of position `from`
+  int64_t ld;     // elements between rows
+  int b0, from, to;  // positions: the block's first, new rows [from, to)
+  int8_t *dst;    // codes of position b0
+  float *scale;
+};
+
+// The bi-th block that entry i's rows touch; false if there is none.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blocks_per_seq) {
+__device__ __forceinline__ bool touched(const AppendArgs &p, int i, int bi, int h, int z, bool tell, Touched<T> &o) {
   const Layer &c = p.c;
-  const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int i = (int)(unit / blocks_per_seq), bi = (int)(unit % blocks_per_seq);
-  if (i >= p.b.m || *c.status) return;
+  if (i >= p.b.m || *c.status) return false;
   const int s = p.b.seq(i, c.n_seqs);
   if (s < 0) {
-    if (lane == 0) atomicOr(c.status, kBadSeq);
-    return;
+    if (tell) atomicOr(c.status, kBadSeq);
+    return false;
   }
   int64_t row0;
   int count;
@@ -48,28 +56,121 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
   const int len = seq_length(c, s), first = len - count;
   // rows before position 0 (more new rows than the sequence holds) are left out
   const int lo = first < 0 ? 0 : first;
-  const int blk = lo / c.block + bi;  // index of this block in the sequence
-  const int b0 = blk * c.block;
-  const int from = lo > b0 ? lo : b0, to = len < b0 + c.block ? len : b0 + c.block;
-  if (from >= to) return;
-  const int pid = c.table[(int64_t)s * c.max_pages + page_of(c, b0)];
+  o.b0 = ((lo >> c.block_shift) + bi) << c.block_shift;
+  o.from = max(lo, o.b0);
+  o.to = min(len, o.b0 + c.block);
+  if (o.from >= o.to) return false;
+  const int pi = page_of(c, o.b0), pid = c.table[(int64_t)s * c.max_pages + pi];
   if ((unsigned)pid >= (unsigned)c.n_pages) {
-    if (lane == 0) atomicOr(c.status, kBadPage);
-    return;
+    if (tell) atomicOr(c.status, kBadPage);
+    return false;
   }
-  const int h = blockIdx.y, z = blockIdx.z;
-  const T *src = (const T *)(z ? p.v : p.k) + (int64_t)h * (z ? p.v_head : p.k_head);
-  const int64_t ld = z ? p.v_row : p.k_row;
-  const int slot0 = b0 - page_of(c, b0) * c.page;
+  o.ld = z ? p.v_row : p.k_row;
+  o.src = (const T *)(z ? p.v : p.k) + h * (z ? p.v_head : p.k_head) + (row0 + o.from - first) * o.ld;
+  const int slot0 = o.b0 - pi * c.page;
   const int64_t ph = (int64_t)pid * c.kv + h;
-  int8_t *dst = (z ? c.v : c.k) + (ph * c.page + slot0) * D;
-  float *sp = (z ? c.vs : c.ks) + ph * (c.page / c.block) + slot0 / c.block;
+  o.dst = (z ? c.v : c.k) + (ph * c.page + slot0) * D;
+  o.scale = (z ? c.vs : c.ks) + ph * (c.page >> c.block_shift) + (slot0 >> c.block_shift);
+  return true;
+}
+
+// Many rows: one block of 128 threads holds the new rows of one touched block
+// in registers (64 rows of 128 f32 are 64 registers a thread), so they are
+// read once, with every load in flight at the same time.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, int blocks_per_seq, int vec) {
+  constexpr int N = 16 / sizeof(T);  // elements of a load
+  constexpr int C = D / N;           // loads of a row
+  constexpr int R = 128 / C;         // rows of one pass
+  constexpr int P = 64 / R;          // passes over a block of 64
+  __shared__ float tops[4];
+  const int tid = threadIdx.x, col = tid % C, row = tid / C;
+  Touched<T> o;
+  if (!touched<T, D>(p, blockIdx.x / blocks_per_seq, blockIdx.x % blocks_per_seq, blockIdx.y, blockIdx.z, tid == 0, o))
+    return;
+  const int n = o.to - o.from;
+  uint4 w[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int r = row + i * R;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (r < n) {
+      const T *src = o.src + r * o.ld + col * N;
+      if (vec) {
+        w[i] = __ldg((const uint4 *)src);
+      } else {
+        T *x = reinterpret_cast<T *>(&w[i]);
+#pragma unroll
+        for (int e = 0; e < N; e++) x[e] = src[e];
+      }
+    }
+  }
+  const float s0 = o.from > o.b0 ? *o.scale : 0.0f;
+  float a = 0.0f;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const T *x = reinterpret_cast<const T *>(&w[i]);
+#pragma unroll
+    for (int e = 0; e < N; e++) a = fmaxf(a, finite_mag(to_f32<T>(x[e])));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, d));
+  if ((tid & 31) == 0) tops[tid >> 5] = a;
+  __syncthreads();
+  a = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float sc = fmaxf(s0, a >= kTiny ? __fmul_rn(a, 1.0f / 127.0f) : 0.0f);
+  const float inv = sc > 0.0f ? __fdiv_rn(1.0f, sc) : 0.0f;
+  if (s0 < sc && o.from > o.b0) {  // the block's older rows
+    const float ratio = __fdiv_rn(s0, sc);
+    for (int x = tid; x < (o.from - o.b0) * (D / 4); x += 128) {
+      char4 q = ((char4 *)o.dst)[x];
+      q.x = (signed char)(int)rintf(__fmul_rn((float)q.x, ratio));
+      q.y = (signed char)(int)rintf(__fmul_rn((float)q.y, ratio));
+      q.z = (signed char)(int)rintf(__fmul_rn((float)q.z, ratio));
+      q.w = (signed char)(int)rintf(__fmul_rn((float)q.w, ratio));
+      ((char4 *)o.dst)[x] = q;
+    }
+  }
+  int8_t *dst = o.dst + (o.from - o.b0) * D + col * N;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int r = row + i * R;
+    if (r >= n) continue;
+    const T *x = reinterpret_cast<const T *>(&w[i]);
+    uint32_t q[N / 4];
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
+      q[e / 4] = (uint32_t)(uint8_t)code_of(to_f32<T>(x[e]), inv) |
+                 (uint32_t)(uint8_t)code_of(to_f32<T>(x[e + 1]), inv) << 8 |
+                 (uint32_t)(uint8_t)code_of(to_f32<T>(x[e + 2]), inv) << 16 |
+                 (uint32_t)(uint8_t)code_of(to_f32<T>(x[e + 3]), inv) << 24;
+    if constexpr (N == 4) {
+      *(uint32_t *)(dst + r * D) = q[0];
+    } else {
+      *(uint2 *)(dst + r * D) = make_uint2(q[0], q[1]);
+    }
+  }
+  if (tid == 0) *o.scale = sc;  // every thread read s0 before the barrier
+}
+
+// Few rows (a step of single tokens, a small chunk): one warp per block.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blocks_per_seq) {
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  Touched<T> o;
+  if (!touched<T, D>(p, (int)(unit / blocks_per_seq), (int)(unit % blocks_per_seq), blockIdx.y, blockIdx.z, lane == 0,
+                     o))
+    return;
+  const int b0 = o.b0, from = o.from, to = o.to;
+  int8_t *dst = o.dst;
+  float *sp = o.scale;
 
   constexpr int E = D / 32;  // elements of a row per lane
   float a = 0.0f;
 #pragma unroll 4
   for (int t = from; t < to; t++) {
-    const T *r = src + (row0 + t - first) * ld + lane * E;
+    const T *r = o.src + (t - from) * o.ld + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e++) a = fmaxf(a, finite_mag(to_f32<T>(r[e])));
   }
@@ -89,7 +190,7 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
   }
 #pragma unroll 4
   for (int t = from; t < to; t++) {
-    const T *r = src + (row0 + t - first) * ld + lane * E;
+    const T *r = o.src + (t - from) * o.ld + lane * E;
     int8_t *d = dst + (t - b0) * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; e++) d[e] = code_of(to_f32<T>(r[e]), inv);
@@ -101,8 +202,17 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
 template <typename T, int D>
 static int launch_append(const AppendArgs &a, cudaStream_t st) {
   const int per = (int)ceil_div(a.b.n - 1, a.c.block) + 1;  // blocks n rows can touch
-  dim3 grid((unsigned)ceil_div((int64_t)a.b.m * per, 4), a.c.kv, 2);
-  append_kernel<T, D><<<grid, 128, 0, st>>>(a, per);
+  if (a.b.n > kStepRows) {
+    auto fits = [](const void *p, int64_t row, int64_t head) {
+      return ((uintptr_t)p | (uintptr_t)(row * (int64_t)sizeof(T)) | (uintptr_t)(head * (int64_t)sizeof(T))) % 16 == 0;
+    };
+    const int vec = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
+    dim3 grid((unsigned)((int64_t)a.b.m * per), a.c.kv, 2);
+    append_block_kernel<T, D><<<grid, 128, 0, st>>>(a, per, vec);
+  } else {
+    dim3 grid((unsigned)ceil_div((int64_t)a.b.m * per, 4), a.c.kv, 2);
+    append_kernel<T, D><<<grid, 128, 0, st>>>(a, per);
+  }
   SC_CUDA(cudaGetLastError());
   note_launch();
   return kOk;
@@ -120,7 +230,8 @@ int append(const AppendArgs &a, cudaStream_t st) {
 
 // ---- reading back --------------------------------------------------------------
 
-// One warp per (row, head): code * scale; tokens without a page read as 0.
+// One warp per token, all its heads (their loads are independent):
+// code * scale; tokens without a page read as 0.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   const Layer &c = p.c;
@@ -135,28 +246,37 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   const int s = p.b.seq(i, c.n_seqs);
   if (s < 0 && lane == 0) atomicOr(c.status, kBadSeq);
   const int tok = s < 0 ? -1 : seq_length(c, s) - count + j;
-  const int pid = tok < 0 ? -1 : c.table[(int64_t)s * c.max_pages + page_of(c, tok)];
+  const int pi = tok < 0 ? 0 : page_of(c, tok);
+  const int pid = tok < 0 ? -1 : c.table[(int64_t)s * c.max_pages + pi];
   const bool ok = (unsigned)pid < (unsigned)c.n_pages;
-  const int h = blockIdx.y, slot = tok < 0 ? 0 : tok - page_of(c, tok) * c.page;
-  const int64_t ph = (int64_t)(ok ? pid : 0) * c.kv + h;
-  constexpr int E = D / 32;
+  const int slot = ok ? tok - pi * c.page : 0, nblk = c.page >> c.block_shift;
+  const int64_t ph = (int64_t)(ok ? pid : 0) * c.kv;
+  constexpr int E = D / 32;  // elements of a head per lane
+  struct alignas(E) Codes { int8_t q[E]; };
+  struct alignas(E * sizeof(T)) Values { T v[E]; };
+#pragma unroll 4
+  for (int h = 0; h < c.kv; h++) {
 #pragma unroll
-  for (int z = 0; z < 2; z++) {
-    T *out = (T *)(z ? p.v : p.k);
-    if (!out) continue;
-    out += ((row0 + j) * c.kv + h) * D + lane * E;
-    float sc = 0.0f;
-    if (ok) sc = (z ? c.vs : c.ks)[ph * (c.page / c.block) + slot / c.block];
-    const int8_t *src = (z ? c.v : c.k) + (ph * c.page + slot) * D + lane * E;
+    for (int z = 0; z < 2; z++) {
+      T *out = (T *)(z ? p.v : p.k);
+      if (!out) continue;
+      Values v;
+      Codes x;
+      float sc = 0.0f;
+      if (ok) {
+        sc = __ldg((z ? c.vs : c.ks) + (ph + h) * nblk + (slot >> c.block_shift));
+        x = *(const Codes *)((z ? c.v : c.k) + ((ph + h) * c.page + slot) * D + lane * E);
+      }
 #pragma unroll
-    for (int e = 0; e < E; e++) out[e] = from_f32<T>(ok ? __fmul_rn((float)src[e], sc) : 0.0f);
+      for (int e = 0; e < E; e++) v.v[e] = from_f32<T>(ok ? __fmul_rn((float)x.q[e], sc) : 0.0f);
+      *(Values *)(out + ((row0 + j) * c.kv + h) * D + lane * E) = v;
+    }
   }
 }
 
 template <typename T, int D>
 static int launch_rows(const RowsArgs &a, cudaStream_t st) {
-  dim3 grid((unsigned)ceil_div((int64_t)a.b.m * a.b.n, 4), a.c.kv);
-  rows_kernel<T, D><<<grid, 128, 0, st>>>(a);
+  rows_kernel<T, D><<<(unsigned)ceil_div((int64_t)a.b.m * a.b.n, 4), 128, 0, st>>>(a);
   SC_CUDA(cudaGetLastError());
   note_launch();
   return kOk;

@@ -172,24 +172,23 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
     tok2 = token(pc.t0 + 2);
     pid2 = page_id(tok2);
     // ---- the rows of q: one warp a row ----
-    for (int r = warp; r < ROWS; r += 4) {
-      float v[D / 32];
+    float qv[ROWS / 4][D / 32];
+#pragma unroll
+    for (int i = 0; i < ROWS / 4; i++) {
+      const int r = warp + 4 * i, row = en.r0 + r, j = row / g.group, hq = pc.head * g.group + row - j * g.group;
+      const T *src = (const T *)p.q + (en.row0 + j) * p.q_row + hq * p.q_head;
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) qv[i][e] = r < nr ? to_f32<T>(src[e * 32 + lane]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS / 4; i++) {
+      const int r = warp + 4 * i;
       float top = 0.0f;
-      if (r < nr) {
-        const int row = en.r0 + r, j = row / g.group, hq = pc.head * g.group + row - j * g.group;
-        const T *src = (const T *)p.q + (en.row0 + j) * p.q_row + hq * p.q_head;
 #pragma unroll
-        for (int e = 0; e < D / 32; e++) {
-          v[e] = to_f32<T>(src[e * 32 + lane]);
-          top = fmaxf(top, fabsf(v[e]));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < D / 32; e++) v[e] = 0.0f;
-      }
+      for (int e = 0; e < D / 32; e++) top = fmaxf(top, fabsf(qv[i][e]));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // 2^k with top * 2^k in [2^13, 2^14); k in [-114, 100] keeps both 2^k and 2^-k normal
+      // 2^k with top * 2^k in [2^13, 2^14); k in [-115, 100] keeps both 2^k and 2^-k normal
       int k = 0;
       if (top > 0.0f) k = min(100, 140 - (int)(__float_as_uint(top) >> 23));
       const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
@@ -200,7 +199,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
         const int d = e * 32 + lane;
         // K step and lane whose registers hold element d of a key
         const int at = (((d >> 6) * 4 + ((d & 15) >> 2)) * 32 + (r & 7) * 4 + ((d & 63) >> 4)) * 4 + (d & 3);
-        const float x = v[e] * up;
+        const float x = qv[i][e] * up;
         const __half h = __float2half_rn(x);
         hi[at] = h;
         if (kSplit) lo[at] = __float2half_rn(x - __half2float(h));
@@ -243,11 +242,16 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
         continue;
       }
       // ---- S^T = K Q^T ----
-      float s[NT][4];
+      // four sums for one tile of rows (two for two): a product waits for the
+      // one before it in its sum
+      constexpr int CH = 4 / NT;
+      float s[NT][4], sp[NT][CH][4];
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] = 0.0f;
+        for (int u = 0; u < CH; u++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sp[n][u][e] = 0.0f;
 #pragma unroll
       for (int f = 0; f < HF; f++) {
         const uint32_t w0[4] = {kr[0][f].x, kr[0][f].y, kr[0][f].z, kr[0][f].w};
@@ -260,14 +264,23 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
 #pragma unroll
           for (int n = 0; n < NT; n++) {
             const uint2 b = sh.q[0][n][f * 4 + j][lane];
-            mma_16816(s[n], a0, a1, a2, a3, b.x, b.y);
             if (kSplit) {
               const uint2 bl = sh.q[1][n][f * 4 + j][lane];
-              mma_16816(s[n], a0, a1, a2, a3, bl.x, bl.y);
+              mma_16816(sp[n][j % (CH / 2)], a0, a1, a2, a3, b.x, b.y);
+              mma_16816(sp[n][CH / 2 + j % (CH / 2)], a0, a1, a2, a3, bl.x, bl.y);
+            } else {
+              mma_16816(sp[n][j % CH], a0, a1, a2, a3, b.x, b.y);
             }
           }
         }
       }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          s[n][e] = sp[n][0][e] + sp[n][1][e];
+          if (CH == 4) s[n][e] += sp[n][CH - 2][e] + sp[n][CH - 1][e];
+        }
       const float kf = ks, vf = vs > 0.0f ? vs : 1.0f;
       load_k(nxt);
       // ---- weights ----
@@ -382,7 +395,10 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       if (p.lse && lane == 0)
         p.lse[(en.row0 + j) * p.n_heads + hq] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
     };
-    for (int r = warp; r < nr; r += 4) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 4; i++) {
+      const int r = warp + 4 * i;
+      if (r >= nr) break;
       float top = -INFINITY, sum = 0.0f, acc[E];
 #pragma unroll
       for (int w = 0; w < 4; w++) top = fmaxf(top, sh.m[w][r]);
