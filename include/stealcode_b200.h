@@ -460,7 +460,8 @@ int sc_rnnt_destroy(sc_rnnt_decoder *r);
  *   status  uint32 [1]      sticky SC_KV8_* bits, 0 at first
  * A new cache has table -1 and length, refs, status 0; codes and scales need
  * no initialisation.  head_dim is 64 or 128; block 16, 32 or 64; page a
- * multiple of block, at most 1024; k and v 16-byte aligned.
+ * multiple of block, at most 1024; k, v and refs 16-byte aligned; at most
+ * 2^30 pages, 2^30 tokens a sequence and 2^20 sequences.
  *
  * A step of some sequences: sc_kv8_reserve (pages for the new tokens; the
  * lengths grow), then per layer sc_kv8_append (their keys and values) and

@@ -34,12 +34,13 @@ int check_cache(const sc_kv8_cache *c) {
   if (c->n_kv_heads < 1 || c->n_kv_heads > 1024) return bad("kv8: n_kv_heads outside 1..1024");
   if (c->n_layers < 1 || c->n_pages < 1 || c->n_seqs < 1 || c->max_pages < 1)
     return bad("kv8: empty cache dimension");
-  if (c->n_pages > INT32_MAX / 2 || c->n_seqs > INT32_MAX / 2 || c->max_pages * (int64_t)c->page > INT32_MAX / 2 ||
+  if (c->n_pages > INT32_MAX / 2 || c->n_seqs > (1 << 20) || c->max_pages * (int64_t)c->page > INT32_MAX / 2 ||
       c->n_seqs > INT32_MAX / c->max_pages || c->max_pages > INT32_MAX / 2)
-    return bad("kv8: cache dimension too large (2^30 pages, tokens a sequence; 2^31 table entries)");
-  if (misaligned(c->k, 16) || misaligned(c->v, 16)) return bad("kv8: k and v have to be 16-byte aligned");
+    return bad("kv8: cache dimension too large (2^30 pages, tokens a sequence; 2^20 sequences; 2^31 table entries)");
+  if (misaligned(c->k, 16) || misaligned(c->v, 16) || misaligned(c->refs, 16))
+    return bad("kv8: k, v and refs have to be 16-byte aligned");
   if (misaligned(c->k_scale, 4) || misaligned(c->v_scale, 4) || misaligned(c->table, 4) || misaligned(c->length, 4) ||
-      misaligned(c->refs, 4) || misaligned(c->status, 4))
+      misaligned(c->status, 4))
     return bad("kv8: misaligned pointer in the cache");
   return kOk;
 }

@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   constexpr int E = D / 32;  // elements of a head per lane
   struct alignas(E) Codes { int8_t q[E]; };
   struct alignas(E * sizeof(T)) Values { T v[E]; };
-#pragma unroll 4
+#pragma unroll 8
   for (int h = 0; h < c.kv; h++) {
 #pragma unroll
     for (int z = 0; z < 2; z++) {

@@ -16,9 +16,12 @@
 // word; while a bit is set, reserve, fork, compact and append do nothing, so
 // a step queued behind a failed one cannot write over a page.  release and
 // slide always run: giving pages back is how a caller recovers.
+#include <atomic>
+
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
+#include "sc_kernels.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -34,7 +37,7 @@ struct PageWs {
   int32_t *head;   // [0] pages to copy, [1] live pages
   int32_t *src, *dst, *used;  // [n_pages] copies: from, to, tokens
   int32_t *map;    // [n_pages] free pages by rank, or a moved page's new id
-  int32_t *off, *len, *claim;  // [n_seqs]
+  int32_t *off, *len;  // [n_seqs]
   int32_t *rows;   // [n_seqs][max_pages] staged table rows
 };
 constexpr int kHeadWords = 64;
@@ -48,13 +51,12 @@ __host__ __device__ static inline PageWs page_ws(void *p, int64_t n_pages, int64
   w.map = w.used + n_pages;
   w.off = w.map + n_pages;
   w.len = w.off + n_seqs;
-  w.claim = w.len + n_seqs;
-  w.rows = w.claim + n_seqs;
+  w.rows = w.len + n_seqs;
   return w;
 }
 
 size_t page_ws_bytes(int64_t n_pages, int64_t n_seqs, int64_t max_pages) {
-  return 4 * (size_t)(kHeadWords + 4 * n_pages + 3 * n_seqs + n_seqs * max_pages);
+  return 4 * (size_t)(kHeadWords + 4 * n_pages + 2 * n_seqs + n_seqs * max_pages);
 }
 
 __device__ __forceinline__ int pages_for(int64_t tokens, int page) { return (int)((tokens + page - 1) / page); }
@@ -123,48 +125,56 @@ __device__ __forceinline__ void page_share(int n_pages, int rank, int *lo, int *
   *hi = (int)(b < n_pages ? b : n_pages);
 }
 
+// Bit e: page p0 + e (of 4, from a multiple of 4) is free and below hi.
+__device__ __forceinline__ unsigned free_bits(const int32_t *refs, int p0, int hi) {
+  if (p0 >= hi) return 0;
+  if (p0 + 4 > hi) {
+    unsigned b = 0;
+    for (int e = 0; p0 + e < hi; e++) b |= (refs[p0 + e] == 0 ? 1u : 0u) << e;
+    return b;
+  }
+  const int4 r = *(const int4 *)(refs + p0);
+  return (r.x == 0 ? 1u : 0u) | (r.y == 0 ? 2u : 0u) | (r.z == 0 ? 4u : 0u) | (r.w == 0 ? 8u : 0u);
+}
+
 // Writes the lowest `need` free pages, ascending, to list (if there are that
 // many); returns the number of free pages of the pool.  All blocks call; the
 // list is complete after the caller's next cluster sync.
 __device__ int list_free(cg::cluster_group cl, PlanShared &sh, const int32_t *refs, int n_pages, int need,
                          int32_t *list) {
+  constexpr int kStrip = 4 * kPlanThreads;
   int lo, hi;
   page_share(n_pages, (int)cl.block_rank(), &lo, &hi);
   int n = 0;
-  for (int p = lo + (int)threadIdx.x; p < hi; p += kPlanThreads) n += refs[p] == 0;
+#pragma unroll 4
+  for (int p = lo + 4 * (int)threadIdx.x; p < hi; p += kStrip) n += __popc(free_bits(refs, p, hi));
   int total, before, all;
   block_scan(n, sh.sums, &total);
   if (threadIdx.x == 0) sh.mine[0] = total;
   cluster_scan(cl, &sh.mine[0], &before, &all);
   if (all >= need) {
-    for (int p0 = lo; p0 < hi && before < need; p0 += kPlanThreads) {
-      const int p = p0 + (int)threadIdx.x;
-      const int f = p < hi && refs[p] == 0;
-      const int r = before + block_scan(f, sh.sums, &total);
-      if (f && r < need) list[r] = p;
+    for (int p0 = lo; p0 < hi && before < need; p0 += kStrip) {
+      const int p = p0 + 4 * (int)threadIdx.x;
+      unsigned f = free_bits(refs, p, hi);
+      int r = before + block_scan(__popc(f), sh.sums, &total);
+      for (; f && r < need; f &= f - 1, r++) list[r] = p + __ffs(f) - 1;
       before += total;
     }
   }
   return all;
 }
 
-// Marks ids that lie outside the cache or are named twice; true if none.
-__device__ bool check_unique(cg::cluster_group cl, PlanShared &sh, const int32_t *seqs, int m, int n_seqs,
-                             int32_t *claim) {
+// True if every id lies in the cache and none is named twice; each block
+// finds out by itself, with a bit for each sequence in shared memory.
+__device__ bool check_unique(const int32_t *seqs, int m, int n_seqs) {
+  extern __shared__ uint32_t named[];
+  if (!seqs) return m <= n_seqs;
+  for (int i = (int)threadIdx.x; i < (n_seqs + 31) / 32; i += kPlanThreads) named[i] = 0;
+  __syncthreads();
   int bad = 0;
-  const int t0 = (int)(cl.block_rank() * kPlanThreads + threadIdx.x), nt = kPlanCtas * kPlanThreads;
-  if (seqs) {
-    for (int i = t0; i < m; i += nt)
-      if ((unsigned)seqs[i] < (unsigned)n_seqs) claim[seqs[i]] = -1;
-    cl.sync();
-    for (int i = t0; i < m; i += nt)
-      if ((unsigned)seqs[i] < (unsigned)n_seqs) atomicMax(&claim[seqs[i]], i);
-    cl.sync();
-    // every block looks at all of them: each decides the same
-    for (int i = (int)threadIdx.x; i < m; i += kPlanThreads)
-      bad |= (unsigned)seqs[i] >= (unsigned)n_seqs || __ldcg(&claim[seqs[i]]) != i;
-  } else {
-    bad = m > n_seqs;
+  for (int i = (int)threadIdx.x; i < m; i += kPlanThreads) {
+    const unsigned s = (unsigned)seqs[i];
+    bad |= s >= (unsigned)n_seqs || (atomicOr(&named[s >> 5], 1u << (s & 31)) >> (s & 31)) & 1u;
   }
   return !__syncthreads_or(bad);
 }
@@ -177,7 +187,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   __shared__ PlanShared sh;
   const PageWs w = page_ws(p.ws, p.n_pages, p.n_seqs);
   if (stopped(cl, sh, p.status)) return;
-  uint32_t fail = check_unique(cl, sh, seqs, m, p.n_seqs, w.claim) ? 0u : (uint32_t)kBadSeq;
+  uint32_t fail = check_unique(seqs, m, p.n_seqs) ? 0u : (uint32_t)kBadSeq;
   // pages each sequence needs, and where its pages start in the list
   int64_t need = 0;
   int wide = 0, negative = 0;
@@ -233,7 +243,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   const bool first = cl.block_rank() == 0 && threadIdx.x == 0;
   if (first) w.head[0] = 0;
   if (stopped(cl, sh, p.status)) return;
-  uint32_t fail = check_unique(cl, sh, children, m, p.n_seqs, w.claim) ? 0u : (uint32_t)kBadSeq;
+  uint32_t fail = check_unique(children, m, p.n_seqs) ? 0u : (uint32_t)kBadSeq;
   int bad = 0;
   for (int i = (int)threadIdx.x; i < m; i += kPlanThreads) bad |= (unsigned)parents[i] >= (unsigned)p.n_seqs;
   if (__syncthreads_or(bad)) fail |= kBadSeq;
@@ -359,33 +369,43 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
 // ---- copying pages ---------------------------------------------------------------
 
 // Copies the listed pages' first used[r] tokens, of every layer and head, K
-// and V: one warp per (page, layer, K or V, head), whose tokens are
-// contiguous.  With `remap` the table's entries follow the moved pages.
+// and V.  A block takes one page of one layer, a warp one head of its K or V,
+// whose tokens are contiguous: eight 16-byte loads a lane before their stores
+// (4 KB a warp in flight).  With `remap` the table's entries follow the moved
+// pages.
 __global__ void __launch_bounds__(256) copy_pages_kernel(const PageArgs p, int remap) {
   const PageWs w = page_ws(p.ws, p.n_pages, p.n_seqs);
   const int n = w.head[0];
-  const int lane = (int)threadIdx.x & 31;
-  const int64_t warps = (int64_t)gridDim.x * 8, warp0 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
   const int per = p.page / p.block;
-  const int64_t units = (int64_t)n * p.n_layers * 2 * p.kv;
-  for (int64_t u = warp0; u < units; u += warps) {
-    const int h = (int)(u % p.kv), z = (int)(u / p.kv % 2);
-    const int64_t l = u / (2 * p.kv) % p.n_layers, r = u / (2 * p.kv) / p.n_layers;
-    const int used = w.used[r];
-    const int64_t a = (l * p.n_pages + w.src[r]) * p.kv + h, b = (l * p.n_pages + w.dst[r]) * p.kv + h;
-    int8_t *c = z ? p.v : p.k;
-    float *s = z ? p.vs : p.ks;
-    const int words = used * (p.head_dim / 16);
-    const uint4 *from = (const uint4 *)(c + a * p.page * p.head_dim);
-    uint4 *to = (uint4 *)(c + b * p.page * p.head_dim);
-    for (int x = lane; x < words; x += 32) to[x] = from[x];
-    const int nb = (used + p.block - 1) / p.block;
-    for (int x = lane; x < nb; x += 32) s[b * per + x] = s[a * per + x];
+  const int64_t all = (int64_t)n * p.n_layers;
+  for (int64_t at = blockIdx.x; at < all; at += gridDim.x) {
+    const int64_t r = at / p.n_layers, l = at - r * p.n_layers;
+    const int used = w.used[r], words = used * (p.head_dim / 16), nb = (used + p.block - 1) / p.block;
+    const int64_t a0 = (l * p.n_pages + w.src[r]) * p.kv, b0 = (l * p.n_pages + w.dst[r]) * p.kv;
+    for (int u = warp; u < 2 * p.kv; u += 8) {
+      const bool z = u >= p.kv;
+      const int64_t a = a0 + (z ? u - p.kv : u), b = b0 + (z ? u - p.kv : u);
+      int8_t *c = z ? p.v : p.k;
+      const uint4 *from = (const uint4 *)(c + a * p.page * p.head_dim);
+      uint4 *to = (uint4 *)(c + b * p.page * p.head_dim);
+      for (int x0 = lane; x0 < words; x0 += 256) {
+        uint4 q[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (x0 + 32 * i < words) q[i] = __ldcs(from + x0 + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (x0 + 32 * i < words) __stcs(to + x0 + 32 * i, q[i]);
+      }
+      float *s = z ? p.vs : p.ks;
+      for (int x = lane; x < nb; x += 32) s[b * per + x] = s[a * per + x];
+    }
   }
   if (remap && n > 0) {
     const int live = w.head[1];
-    const int64_t all = (int64_t)p.n_seqs * p.max_pages, threads = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < all; e += threads) {
+    const int64_t entries = (int64_t)p.n_seqs * p.max_pages, threads = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < entries; e += threads) {
       const int pid = p.table[e];
       if (pid >= live && pid < p.n_pages) p.table[e] = w.map[pid];
     }
@@ -430,8 +450,14 @@ __global__ void __launch_bounds__(128) slide_kernel(const PageArgs p, const int3
 
 // ---- launches ----------------------------------------------------------------------
 
+// Shared memory of a plan: one bit for each sequence.
+static size_t named_bytes(const PageArgs &a) { return (size_t)ceil_div(a.n_seqs, 32) * 4; }
+
 int reserve(const PageArgs &a, const int32_t *seqs, const int32_t *counts, int m, cudaStream_t st) {
-  reserve_kernel<<<kPlanCtas, kPlanThreads, 0, st>>>(a, seqs, counts, m);
+  static std::atomic<size_t> limit[64];
+  const int rc = raise_smem_limit((const void *)reserve_kernel, named_bytes(a), limit);
+  if (rc) return rc;
+  reserve_kernel<<<kPlanCtas, kPlanThreads, named_bytes(a), st>>>(a, seqs, counts, m);
   SC_CUDA(cudaGetLastError());
   note_launch();
   return kOk;
@@ -445,7 +471,10 @@ static int copy_pages(const PageArgs &a, int remap, int sm_count, cudaStream_t s
 }
 
 int fork(const PageArgs &a, const int32_t *parents, const int32_t *children, int m, int sm_count, cudaStream_t st) {
-  fork_kernel<<<kPlanCtas, kPlanThreads, 0, st>>>(a, parents, children, m);
+  static std::atomic<size_t> limit[64];
+  const int rc = raise_smem_limit((const void *)fork_kernel, named_bytes(a), limit);
+  if (rc) return rc;
+  fork_kernel<<<kPlanCtas, kPlanThreads, named_bytes(a), st>>>(a, parents, children, m);
   SC_CUDA(cudaGetLastError());
   note_launch();
   return copy_pages(a, 0, sm_count, st);
