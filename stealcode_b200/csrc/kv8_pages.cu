@@ -223,10 +223,18 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     const int64_t len = p.length[s], end = len + counts[i];
     const int have = pages_for(len, p.page), n = pages_for(end, p.page) - have;
     const int off = __ldcg(&w.off[i]);
-    for (int j = lane; j < n; j += 32) {
-      const int pid = __ldcg(&w.map[off + j]);
-      p.table[(int64_t)s * p.max_pages + have + j] = pid;
-      p.refs[pid] = 1;
+    int32_t *row = p.table + (int64_t)s * p.max_pages + have;
+    for (int j0 = lane; j0 < n; j0 += 256) {
+      int pid[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (j0 + 32 * e < n) pid[e] = __ldcg(&w.map[off + j0 + 32 * e]);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (j0 + 32 * e < n) {
+          row[j0 + 32 * e] = pid[e];
+          p.refs[pid[e]] = 1;
+        }
     }
     __syncwarp();
     if (lane == 0) p.length[s] = (int)end;

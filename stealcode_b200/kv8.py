@@ -22,6 +22,7 @@ the host; failures that only the device sees (too few free pages) are read with
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from ctypes import c_int32, c_int64, c_void_p
 
@@ -46,6 +47,9 @@ _FAILURES = (
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+_NO_STREAM = contextlib.nullcontext()
 
 
 class _Cache(ctypes.Structure):
@@ -119,13 +123,6 @@ class KvCache8:
             raise ValueError(f"the cache lives on {self.device}, the current device is {_current_device()}")
         return _raw_stream(self._index) if stream is None else stream.cuda_stream
 
-    def _empty(self, stream, *args, **kw):
-        """torch.empty on the stream that will use it."""
-        if stream is None:
-            return torch.empty(*args, device=self.device, **kw)
-        with torch.cuda.stream(stream):
-            return torch.empty(*args, device=self.device, **kw)
-
     def _ids(self, t, name: str) -> int:
         if t is None:
             return 0
@@ -191,8 +188,10 @@ class KvCache8:
         if dtype not in _DTYPES:
             raise ValueError("dtype has to be f32, f16 or bf16")
         st = self._stream(stream)
-        shape = (b.total, self.n_kv_heads, self.head_dim)
-        k, v = self._empty(stream, shape, dtype=dtype), self._empty(stream, shape, dtype=dtype)
+        # allocations belong to the stream that uses them
+        with _NO_STREAM if stream is None else torch.cuda.stream(stream):
+            k = self.k_scale.new_empty((b.total, self.n_kv_heads, self.head_dim), dtype=dtype)
+            v = torch.empty_like(k)
         rc = lib.sc_kv8_rows(self._p, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], st)
         if rc:
             check(rc)
@@ -212,13 +211,14 @@ class KvCache8:
         self._rows_in(q, heads, "q")
         b = self._batch(seqs, cu, n, q.shape[0])
         st = self._stream(stream)
-        if out is None:
-            out = self._empty(stream, q.shape, dtype=q.dtype)
-        else:
+        if out is not None:
             self._rows_in(out, heads, "out")
             if out.dtype != q.dtype or out.shape != q.shape:
                 raise ValueError("out has to have q's type and shape")
-        lse = self._empty(stream, q.shape[:2], dtype=torch.float32) if return_lse else None
+        with _NO_STREAM if stream is None else torch.cuda.stream(stream):
+            if out is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            lse = self.k_scale.new_empty((q.shape[0], heads)) if return_lse else None
         ws = self._workspace("attend", st, stream, lib.sc_kv8_attend_workspace_bytes)
         qs, os_ = q.stride(), out.stride()
         rc = lib.sc_kv8_attend(self._p, layer, ctypes.byref(b), q.data_ptr(), qs[0], qs[1], heads,
