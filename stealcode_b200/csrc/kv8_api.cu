@@ -37,6 +37,8 @@ int check_cache(const sc_kv8_cache *c) {
   if (c->n_pages > INT32_MAX / 2 || c->n_seqs > (1 << 20) || c->max_pages * (int64_t)c->page > INT32_MAX / 2 ||
       c->n_seqs > INT32_MAX / c->max_pages || c->max_pages > INT32_MAX / 2)
     return bad("kv8: cache dimension too large (2^30 pages, tokens a sequence; 2^20 sequences; 2^31 table entries)");
+  if (c->max_pages * (int64_t)c->page / 16 * c->n_kv_heads > INT32_MAX)  // work units of one sequence
+    return bad("kv8: more than 2^35 tokens x kv heads in one sequence");
   if (misaligned(c->k, 16) || misaligned(c->v, 16) || misaligned(c->refs, 16))
     return bad("kv8: k, v and refs have to be 16-byte aligned");
   if (misaligned(c->k_scale, 4) || misaligned(c->v_scale, 4) || misaligned(c->table, 4) || misaligned(c->length, 4) ||
@@ -184,7 +186,8 @@ int sc_kv8_attend(const sc_kv8_cache *c, int64_t layer, const sc_kv8_batch *b, c
     a.sinks = (int)(sinks < most ? sinks : most);
   }
   const int64_t group = n_heads / c->n_kv_heads;
-  if (b->m * (b->n * group / 8 + 1) > INT32_MAX / 2) return bad("kv8_attend: too many query rows");
+  if (b->n * group > INT32_MAX / 2 || b->m * (b->n * group / 8 + 1) > INT32_MAX / 2)
+    return bad("kv8_attend: too many query rows");
   return kv8::attend(a, sms, (cudaStream_t)stream);
 }
 

@@ -175,8 +175,10 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
     float qv[ROWS / 4][D / 32];
 #pragma unroll
     for (int i = 0; i < ROWS / 4; i++) {
-      const int r = warp + 4 * i, row = en.r0 + r, j = row / g.group, hq = pc.head * g.group + row - j * g.group;
-      const T *src = (const T *)p.q + (en.row0 + j) * p.q_row + hq * p.q_head;
+      const int r = warp + 4 * i;
+      int j, h;
+      en.row(g, r, j, h);
+      const T *src = (const T *)p.q + (en.row0 + j) * p.q_row + (pc.head * g.group + h) * p.q_head;
 #pragma unroll
       for (int e = 0; e < D / 32; e++) qv[i][e] = r < nr ? to_f32<T>(src[e * 32 + lane]) : 0.0f;
     }
@@ -213,7 +215,9 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int r = n * 8 + 2 * ti + u;
-        pos[n][u] = r < nr ? en.first + (en.r0 + r) / g.group : -1;
+        int j, h;
+        en.row(g, r, j, h);
+        pos[n][u] = r < nr ? en.first + j : -1;
         qf[n][u] = sh.qf[r];
       }
 
@@ -387,7 +391,9 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
     // a warp takes a row, a lane D / 32 of its elements
     constexpr int E = D / 32;
     auto store = [&](int r, float top, float sum, const float (&acc)[E]) {
-      const int row = en.r0 + r, j = row / g.group, hq = pc.head * g.group + row - j * g.group;
+      int j, hq;
+      en.row(g, r, j, hq);
+      hq += pc.head * g.group;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kShift);
       T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
 #pragma unroll
@@ -471,6 +477,7 @@ static int launch_step(const AttendArgs &a, int sm_count, cudaStream_t st) {
   constexpr int ROWS = 8 * NT;
   WorkGrid g;
   g.group = a.n_heads / a.c.kv;
+  g.magic = (uint32_t)((2097152 + g.group - 1) / g.group);
   g.per_seq = (int)ceil_div((int64_t)a.b.n * g.group, ROWS);
   g.entries = a.b.m * g.per_seq;
   // A share of u tiles takes about 0.6 us a tile, joining a past of n tiles

@@ -13,8 +13,13 @@
 //                   in registers) and write them to shared memory as f16
 //                   operands: K as it lies (its depth is contiguous), V
 //                   transposed by stmatrix;
-//   warp 20         issues S = Q K^T and O += W V; while one row tile is in
-//                   its softmax the other's products run.
+//   warps 20, 21    issue S = Q K^T and O += W V of row tile 0, 1: while one
+//                   row tile is in its softmax the other's products run.  A
+//                   warp each, since a row tile's chain (softmax, W V, the
+//                   next Q K^T over the weights just read) waits for a barrier
+//                   at every step and one warp would wait for both in turn;
+//   warp 22         runs one piece ahead and sends its queries and first keys
+//                   to L2.
 // The codes pass through the converters once for 256 rows, so their cost is
 // shared by all query heads of the group.
 //
@@ -33,7 +38,7 @@ namespace sc {
 namespace kv8 {
 
 constexpr int kTileRows = 256, kTileKeys = 128;
-constexpr int kTileThreads = 768;  // 21 warps work; setmaxnreg takes whole warpgroups
+constexpr int kTileThreads = 768;  // 23 warps work; setmaxnreg takes whole warpgroups
 constexpr int kTileOver = 3;  // an item's queries and result cost about as much as three tiles
 constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
 constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
@@ -59,6 +64,7 @@ struct TileShared {  // after the operands
   ShareScratch share;
   uint32_t tmem;
   int last;
+  volatile int started;  // pieces the softmax warps have begun
 };
 
 __device__ __forceinline__ bool elect_one() {
@@ -69,6 +75,8 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
+// The eight warps of a row tile.
+__device__ __forceinline__ void tile_sync(int q) { asm volatile("bar.sync %0, 256;" ::"r"(10 + q) : "memory"); }
 // The two warps that hold the halves of 32 rows.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
@@ -225,15 +233,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   Share share;
   if (!find_share<kTileRows, kTileKeys, kTileOver, kTileThreads>(p, g, sh.share, share)) return;
   if (tid == 0) {
+    sh.started = 0;
     for (int i = 0; i < 2; i++) {
       mbar_init(&sh.q_full[i], 8);
       mbar_init(&sh.s_full[i], 2);  // the MMA thread's own arrival and its commit
       mbar_init(&sh.p_full[i], 8);
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.k_full[i], 4);
-      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.k_empty[i], 2);  // both MMA warps
       mbar_init(&sh.v_full[i], 4);
-      mbar_init(&sh.v_empty[i], 1);
+      mbar_init(&sh.v_empty[i], 2);
     }
     fence_barrier_init();
   }
@@ -267,18 +276,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const bool on = q * 128 < nr;          // this row tile has rows
       const int r = en.r0 + q * 128 + row;   // row of the sequence
       const bool mine = r < en.r1;
-      const int j = r / g.group, hq = pc.head * g.group + r - j * g.group;
+      int j, hq;
+      en.row(g, q * 128 + row, j, hq);
+      hq += pc.head * g.group;
       const int pos = mine ? en.first + j : -1;
       float m = -INFINITY, l = 0.0f;
+      if (tid == 0) sh.started = sh.started + 1;
       if (on && nt > 0) {
         // the pair of warps loads its 32 rows, 16 each
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
           const int lr = (warp & 3) * 32 + half * 16 + i * 8 + (lane & 7), r2 = en.r0 + q * 128 + lr;
-          const int j2 = r2 / g.group, h2 = pc.head * g.group + r2 - j2 * g.group;
+          int j2, h2;
+          en.row(g, q * 128 + lr, j2, h2);
           unsigned char *hi = qs + q * C::kTerms * C::kQ + lr * 16;
-          load_queries<D, T>(r2 < en.r1 ? (const T *)p.q + (en.row0 + j2) * p.q_row + h2 * p.q_head : nullptr, vec_q,
-                             p.scale, hi, hi + C::kQ, &sh.top[1][q][0][lr]);
+          load_queries<D, T>(
+              r2 < en.r1 ? (const T *)p.q + (en.row0 + j2) * p.q_row + (pc.head * g.group + h2) * p.q_head : nullptr,
+              vec_q, p.scale, hi, hi + C::kQ, &sh.top[1][q][0][lr]);
         }
         pair_sync(pair);
         const float qf = sh.top[1][q][0][row];
@@ -286,8 +300,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.q_full[q]);
         // positions of the row tile's first and last row
-        const int p_lo = en.first + (en.r0 + q * 128) / g.group;
-        const int p_hi = en.first + (min(en.r1, en.r0 + q * 128 + 128) - 1) / g.group;
+        int j_lo, j_hi, h_any;
+        en.row(g, q * 128, j_lo, h_any);
+        en.row(g, min(nr, q * 128 + 128) - 1, j_hi, h_any);
+        const int p_lo = en.first + j_lo, p_hi = en.first + j_hi;
         for (int x = 0; x < nt; x++, ns++) {
           if (ok) ok = mbar_wait(&sh.s_full[q], (uint32_t)ns & 1u);
           __syncwarp();
@@ -417,6 +433,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int pr = q * 128 + row;  // row of the item
         const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / (l * kTileShift)) : 1.0f;
         T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
+        // A whole item's rows go through the queries' shared memory (their
+        // last product has completed), 16-byte pieces swizzled by the row, so
+        // that both the writes here and the rows' stores below run over whole
+        // lines: a thread's own row would be a line for each lane.
+        constexpr int RB = D * sizeof(T);  // bytes of a row
+        unsigned char *stage = qs + q * C::kTerms * C::kQ;
+        const bool staged = pc.whole && vec_o;
+        if (staged) tile_sync(q);  // no warp still reads the queries' sums or stages of the piece before
 #pragma unroll 1
         for (int i = half * (D / 64); i < (half + 1) * (D / 64); i++) {
           uint32_t o[32];
@@ -427,21 +451,48 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; e++) o[e] = 0;
           }
-          if (mine) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) {  // 8 consecutive elements
-              float v[8];
+          for (int t = 0; t < 4; t++) {  // 8 consecutive elements
+            float v[8];
 #pragma unroll
-              for (int e = 0; e < 8; e++) v[e] = __uint_as_float(o[8 * (e / 2) + 2 * t + (e & 1)]) * inv;
-              const int d0 = (i >> 1) * 64 + t * 16 + (i & 1) * 8;
+            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(o[8 * (e / 2) + 2 * t + (e & 1)]) * inv;
+            const int d0 = (i >> 1) * 64 + t * 16 + (i & 1) * 8;
+            if (staged) {
+              constexpr int W = 16 / sizeof(T);
+#pragma unroll
+              for (int e = 0; e < 8; e += W) {
+                uint4 w;
+                T *x = reinterpret_cast<T *>(&w);
+#pragma unroll
+                for (int u = 0; u < W; u++) x[u] = from_f32<T>(v[e + u]);
+                *(uint4 *)(stage + row * RB + ((((d0 + e) / W) ^ (row & 7)) * 16)) = w;
+              }
+            } else if (mine) {
               if (!pc.whole) {
                 *(float4 *)(part + (int64_t)pr * D + d0) = make_float4(v[0], v[1], v[2], v[3]);
                 *(float4 *)(part + (int64_t)pr * D + d0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
               } else {
-                store_row<T, 8>(dst + d0, v, vec_o);
+#pragma unroll
+                for (int e = 0; e < 8; e++) dst[d0 + e] = from_f32<T>(v[e]);
               }
             }
           }
+        }
+        if (staged) {
+          pair_sync(pair);
+          constexpr int L = RB / 16;  // lanes of a row
+#pragma unroll 4
+          for (int i = 0; i < 16; i += 32 / L) {
+            const int lr = (warp & 3) * 32 + half * 16 + i + lane / L, r2 = en.r0 + q * 128 + lr;
+            if (r2 < en.r1) {
+              int j2, h2;
+              en.row(g, q * 128 + lr, j2, h2);
+              const uint4 w = *(const uint4 *)(stage + lr * RB + (((lane % L) ^ (lr & 7)) * 16));
+              *(uint4 *)((T *)p.out + (en.row0 + j2) * p.o_row + (pc.head * g.group + h2) * p.o_head +
+                         (lane % L) * (16 / sizeof(T))) = w;
+            }
+          }
+          tile_sync(q);  // the next piece's queries may be written
         }
         if (mine && half == 0) {
           if (pc.whole) {
@@ -488,7 +539,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 acc[4 * e + 3] += f * v.w;
               }
             }
-            const int r2 = en.r0 + rr, j2 = r2 / g.group, h2 = pc.head * g.group + r2 - j2 * g.group;
+            int j2, h2;
+            en.row(g, rr, j2, h2);
+            h2 += pc.head * g.group;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kTileShift);
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
@@ -640,16 +693,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   } else {
     // ================= MMA =================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == 20) {
+    if (warp < 22) {
       // the whole warp walks the tiles (so that addresses stay in uniform
-      // registers), one lane issues
+      // registers) and polls the barriers, one lane issues
       const bool lead = elect_one();
+      const int q = __shfl_sync(0xffffffffu, warp - 20, 0);
       const uint32_t id_s = umma_idesc_f16(128), id_o = umma_idesc_f16(D);
-      const uint64_t q0 = umma_desc(qs, 2048, 128), k0 = umma_desc(kt, 2048, 128), v0 = umma_desc(vt, D * 16, 128);
-      int np0 = 0, np1 = 0, nq0 = 0, nq1 = 0, nk = 0;  // products into O, pieces of each row tile, key tiles
-      // S of row tile q from K stage st, once the last product that read its
-      // weights (they lie over the scores) has completed
-      auto scores = [&](int q, int np, int st, bool last) {
+      const uint64_t qd = umma_desc(qs + q * C::kTerms * C::kQ, 2048, 128), k0 = umma_desc(kt, 2048, 128),
+                     v0 = umma_desc(vt, D * 16, 128);
+      const uint32_t s_at = tmem + q * 128, o_at = tmem + 256 + q * 128;
+      int np = 0, nq = 0, nk = 0;  // products into O, pieces with this row tile, key tiles
+      // S from K stage st, once the last product that read its weights (they
+      // lie over the scores) has completed
+      auto scores = [&](int x) {
+        const int st = (nk + x) % NS;
+        if (!mbar_wait(&sh.k_full[st], (uint32_t)((nk + x) / NS) & 1u)) return false;
         if (np > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np - 1) & 1u)) return false;
         tc_fence_after();
         if (lead) {
@@ -658,15 +716,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int t = 0; t < C::kTerms; t++)  // low terms first: less of them is lost to the large sums
 #pragma unroll
             for (int i = 0; i < D / 16; i++)
-              tc_mma_f16(tmem + q * 128, q0 + (uint64_t)(((q * C::kTerms + C::kTerms - 1 - t) * C::kQ + i * 4096) >> 4),
+              tc_mma_f16(s_at, qd + (uint64_t)(((C::kTerms - 1 - t) * C::kQ + i * 4096) >> 4),
                          kd + (uint64_t)((i * 4096) >> 4), id_s, (uint32_t)(t | i));
           mbar_arrive(&sh.s_full[q]);
           tc_commit(&sh.s_full[q]);
-          if (last) tc_commit(&sh.k_empty[st]);
+          tc_commit(&sh.k_empty[st]);
         }
         return true;
       };
-      auto output = [&](int q, int np, int st, bool first, bool last) {
+      auto output = [&](int x) {
+        const int st = (nk + x) % NS;
+        if (!mbar_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u)) return false;
         if (!mbar_wait(&sh.p_full[q], (uint32_t)np & 1u)) return false;
         tc_fence_after();
         if (lead) {
@@ -675,41 +735,62 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int t = 0; t < C::kTerms; t++)
 #pragma unroll
             for (int i = 0; i < 8; i++)
-              tc_mma_ts(tmem + 256 + q * 128, tmem + q * 128 + (i >> 1) * 32 + t * 16 + (i & 1) * 8,
-                        vd + (uint64_t)((i * 2 * D * 16) >> 4), id_o, t | i ? 1u : first ? 0u : 1u);
+              tc_mma_ts(o_at, s_at + (i >> 1) * 32 + t * 16 + (i & 1) * 8, vd + (uint64_t)((i * 2 * D * 16) >> 4), id_o,
+                        t | i ? 1u : (uint32_t)x);
           tc_commit(&sh.pv_done[q]);
-          if (last) tc_commit(&sh.v_empty[st]);
+          tc_commit(&sh.v_empty[st]);
         }
         return true;
       };
       while (ok && next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
         const int nt = max(0, min(pc.t1, en.tiles()) - pc.t0);
         if (nt == 0) continue;
-        const bool two = en.r1 - en.r0 > 128;
-        ok = mbar_wait(&sh.q_full[0], (uint32_t)nq0++ & 1u) && mbar_wait(&sh.k_full[nk % NS], (uint32_t)(nk / NS) & 1u) &&
-             scores(0, np0, nk % NS, !two);
-        if (ok && two) ok = mbar_wait(&sh.q_full[1], (uint32_t)nq1++ & 1u) && scores(1, np1, nk % NS, true);
-        ok = __all_sync(0xffffffffu, ok);  // lanes poll by themselves; one that gave up ends the loop for all
-        for (int x = 0; x < nt && ok; x++) {
-          // O += W V of tile x, then S of tile x + 1: first one row tile, then the other
-          const int st = (nk + x) % NS, st1 = (nk + x + 1) % NS;
-          const bool more = x + 1 < nt;
-          ok = mbar_wait(&sh.v_full[st], (uint32_t)((nk + x) / NS) & 1u) && output(0, np0, st, x == 0, !two);
-          np0++;
-          if (ok && more)
-            ok = mbar_wait(&sh.k_full[st1], (uint32_t)((nk + x + 1) / NS) & 1u) && scores(0, np0, st1, !two);
-          if (ok && two) {
-            ok = output(1, np1, st, x == 0, true);
-            np1++;
-            if (ok && more) ok = scores(1, np1, st1, true);
+        if (q == 0 || en.r1 - en.r0 > 128) {
+          ok = mbar_wait(&sh.q_full[q], (uint32_t)nq++ & 1u) && scores(0);
+          for (int x = 0; x < nt && ok; x++) {
+            ok = output(x);
+            np++;
+            if (ok && x + 1 < nt) ok = scores(x + 1);
+            ok = __all_sync(0xffffffffu, ok);  // a lane whose wait gave up ends the loop for all
           }
-          ok = __all_sync(0xffffffffu, ok);
+        } else {  // no rows here: the tiles are released unread
+          for (int x = 0; x < nt && ok; x++) {
+            const int st = (nk + x) % NS;
+            const uint32_t turn = (uint32_t)((nk + x) / NS) & 1u;
+            ok = mbar_wait(&sh.k_full[st], turn);
+            if (ok && lead) mbar_arrive(&sh.k_empty[st]);
+            ok = ok && mbar_wait(&sh.v_full[st], turn);
+            if (ok && lead) mbar_arrive(&sh.v_empty[st]);
+            ok = __all_sync(0xffffffffu, ok);
+          }
         }
+        ok = __all_sync(0xffffffffu, ok);
         nk += nt;
       }
       // every product completes before the tensor memory is released
-      if (np0 > 0 && !mbar_wait(&sh.pv_done[0], (uint32_t)(np0 - 1) & 1u)) ok = false;
-      if (np1 > 0 && !mbar_wait(&sh.pv_done[1], (uint32_t)(np1 - 1) & 1u)) ok = false;
+      if (np > 0 && !mbar_wait(&sh.pv_done[q], (uint32_t)(np - 1) & 1u)) ok = false;
+    }
+    if (warp == 22) {
+      int n = 0;
+      const long long t0 = clock64();
+      while (next_piece<kTileRows, kTileKeys, kTileOver>(p, g, share, en, pc)) {
+        // one piece ahead of the softmax warps; a hint only, so it gives up quietly
+        while (sh.started < n && clock64() - t0 < kWaitCycles) __nanosleep(200);
+        n++;
+        if (pc.t0 >= en.tiles()) continue;
+        if (vec_q)
+          for (int r = en.r0 + lane; r < en.r1; r += 32) {
+            int j, h;
+            en.row(g, r - en.r0, j, h);
+            prefetch_l2((const T *)p.q + (en.row0 + j) * p.q_row + (pc.head * g.group + h) * p.q_head, D * sizeof(T));
+          }
+        const int tok = en.tile(pc.t0) * kTileKeys + (lane >> 1) * 16, pi = page_of(c, tok);
+        if (lane < 16 && tok <= en.p_hi) {
+          const int pid = c.table[(int64_t)en.s * c.max_pages + pi];
+          if ((unsigned)pid < (unsigned)c.n_pages)
+            prefetch_l2((lane & 1 ? c.v : c.k) + (((int64_t)pid * c.kv + pc.head) * c.page + tok - pi * c.page) * D, 16 * D);
+        }
+      }
     }
     __syncwarp();
   }
@@ -726,6 +807,7 @@ static int launch_tile(const AttendArgs &a, int sm_count, cudaStream_t st) {
   using C = TileCfg<D, sizeof(T) == 4>;
   WorkGrid g;
   g.group = a.n_heads / a.c.kv;
+  g.magic = (uint32_t)((2097152 + g.group - 1) / g.group);
   g.per_seq = (int)ceil_div((int64_t)a.b.n * g.group, kTileRows);
   g.entries = a.b.m * g.per_seq;
   g.min_share = 2;

@@ -20,6 +20,7 @@ namespace kv8 {
 
 struct WorkGrid {
   int group;       // query heads per kv head
+  uint32_t magic;  // 2^21 / group, rounded up
   int per_seq;     // items per sequence and kv head, at most
   int entries;     // m * per_seq
   int min_share;   // units; fewer blocks work when there are few
@@ -32,17 +33,25 @@ struct Entry {
   int64_t row0;     // first packed token
   int first;        // position of that token
   int r0, r1;       // rows [r0, r1) of the sequence
+  int j0, h0;       // row r0's token (from row0) and query head
   int p_lo, p_hi;   // positions of the first and the last row
   int a, b, c;
   __device__ __forceinline__ int tiles() const { return a + c - b; }
   __device__ __forceinline__ int steps() const { return max(1, tiles()); }  // an item without keys has a result too
   __device__ __forceinline__ int tile(int x) const { return x < a ? x : b + x - a; }
+  // Token and query head of row r0 + k, k < 256: (h0 + k) / group by a product
+  // with 2^21 / group rounded up, exact as (h0 + k) * group < 1280 * 1024 < 2^21.
+  __device__ __forceinline__ void row(const WorkGrid &g, int k, int &j, int &h) const {
+    const uint32_t x = (uint32_t)(h0 + k), d = x * g.magic >> 21;
+    j = j0 + (int)d;
+    h = (int)(x - d * (uint32_t)g.group);
+  }
 };
 
 // False when entry e has no rows.
 template <int ROWS, int TILE>
 __device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g, int e, Entry &o) {
-  o.i = e / g.per_seq;
+  o.i = (int)((uint32_t)e / (uint32_t)g.per_seq);
   int count;
   p.b.rows(o.i, o.row0, count);
   o.r0 = (e - o.i * g.per_seq) * ROWS;
@@ -52,8 +61,12 @@ __device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g
   o.s = p.b.seq(o.i, p.c.n_seqs);
   const int len = o.s < 0 ? 0 : seq_length(p.c, o.s);
   o.first = len - count;
-  o.p_lo = o.first + o.r0 / g.group;
-  o.p_hi = o.first + (o.r1 - 1) / g.group;
+  o.j0 = (int)((uint32_t)o.r0 / (uint32_t)g.group);
+  o.h0 = o.r0 - o.j0 * g.group;
+  int j, h;
+  o.row(g, o.r1 - 1 - o.r0, j, h);
+  o.p_lo = o.first + o.j0;
+  o.p_hi = o.first + j;
   o.a = o.b = o.c = 0;
   if (o.p_hi >= 0) {
     o.c = o.p_hi / TILE + 1;
@@ -159,7 +172,7 @@ __device__ __forceinline__ bool next_piece(const AttendArgs &p, const WorkGrid &
       o.e++;
       continue;
     }
-    q.head = (int)((o.pos - o.at) / cost);
+    q.head = (int)((uint32_t)(o.pos - o.at) / (uint32_t)cost);
     const int64_t s0 = o.at + (int64_t)q.head * cost + OVER;  // unit of tile 0
     const int64_t end = o.end < s0 + steps ? o.end : s0 + steps;
     q.t0 = o.pos > s0 ? (int)(o.pos - s0) : 0;
