@@ -33,44 +33,56 @@ __device__ __forceinline__ int8_t code_of(float x, float inv) {
 // One touched block of one head, of K (z = 0) or V (z = 1).
 template <typename T>
 struct Touched {
-  const T *src;   // the row of position `from`
-  int64_t ld;     // elements between rows
+  const T *src;      // the row of position `from`
+  int64_t ld;        // elements between rows
+  int s, h, z;
   int b0, from, to;  // positions: the block's first, new rows [from, to)
-  int8_t *dst;    // codes of position b0
+  int8_t *dst;       // codes of position b0
   float *scale;
 };
 
-// The bi-th block that entry i's rows touch; false if there is none.
-template <typename T, int D>
-__device__ __forceinline__ bool touched(const AppendArgs &p, int i, int bi, int h, int z, bool tell, Touched<T> &o) {
+// The bi-th block that entry i's rows touch; false if there is none.  Its
+// rows can be loaded then; find_page says where they go.  (The status word
+// and the page table are read behind the rows: each would be a round trip to
+// memory before the first of them.)
+template <typename T>
+__device__ __forceinline__ bool find_rows(const AppendArgs &p, int i, int bi, int h, int z, bool tell, Touched<T> &o) {
   const Layer &c = p.c;
-  if (i >= p.b.m || *c.status) return false;
-  const int s = p.b.seq(i, c.n_seqs);
-  if (s < 0) {
+  if (i >= p.b.m) return false;
+  o.s = p.b.seq(i, c.n_seqs);
+  if (o.s < 0) {
     if (tell) atomicOr(c.status, kBadSeq);
     return false;
   }
   int64_t row0;
   int count;
   p.b.rows(i, row0, count);
-  const int len = seq_length(c, s), first = len - count;
+  const int len = seq_length(c, o.s), first = len - count;
   // rows before position 0 (more new rows than the sequence holds) are left out
   const int lo = first < 0 ? 0 : first;
   o.b0 = ((lo >> c.block_shift) + bi) << c.block_shift;
   o.from = max(lo, o.b0);
   o.to = min(len, o.b0 + c.block);
   if (o.from >= o.to) return false;
-  const int pi = page_of(c, o.b0), pid = c.table[(int64_t)s * c.max_pages + pi];
+  o.h = h;
+  o.z = z;
+  o.ld = z ? p.v_row : p.k_row;
+  o.src = (const T *)(z ? p.v : p.k) + h * (z ? p.v_head : p.k_head) + (row0 + o.from - first) * o.ld;
+  return true;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ bool find_page(const Layer &c, bool tell, Touched<T> &o) {
+  const int pi = page_of(c, o.b0), pid = c.table[(int64_t)o.s * c.max_pages + pi];
+  if (*c.status) return false;
   if ((unsigned)pid >= (unsigned)c.n_pages) {
     if (tell) atomicOr(c.status, kBadPage);
     return false;
   }
-  o.ld = z ? p.v_row : p.k_row;
-  o.src = (const T *)(z ? p.v : p.k) + h * (z ? p.v_head : p.k_head) + (row0 + o.from - first) * o.ld;
   const int slot0 = o.b0 - pi * c.page;
-  const int64_t ph = (int64_t)pid * c.kv + h;
-  o.dst = (z ? c.v : c.k) + (ph * c.page + slot0) * D;
-  o.scale = (z ? c.vs : c.ks) + ph * (c.page >> c.block_shift) + (slot0 >> c.block_shift);
+  const int64_t ph = (int64_t)pid * c.kv + o.h;
+  o.dst = (o.z ? c.v : c.k) + (ph * c.page + slot0) * D;
+  o.scale = (o.z ? c.vs : c.ks) + ph * (c.page >> c.block_shift) + (slot0 >> c.block_shift);
   return true;
 }
 
@@ -78,16 +90,41 @@ __device__ __forceinline__ bool touched(const AppendArgs &p, int i, int bi, int 
 // in registers (64 rows of 128 f32 are 64 registers a thread), so they are
 // read once, with every load in flight at the same time.
 template <typename T, int D>
+//
+// Uneven rows (cu): entry i's touched blocks take the slots from
+// cu[i] / block + 2 i, which leaves room for one more block at either end, so
+// the grid has total / block + 2 m slots instead of m times the longest
+// entry's; a block of threads finds its entry with one load a thread.
 __global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, int blocks_per_seq, int vec) {
   constexpr int N = 16 / sizeof(T);  // elements of a load
   constexpr int C = D / N;           // loads of a row
   constexpr int R = 128 / C;         // rows of one pass
   constexpr int P = 64 / R;          // passes over a block of 64
   __shared__ float tops[4];
+  __shared__ int found[2];
   const int tid = threadIdx.x, col = tid % C, row = tid / C;
+  // the heads of K and V are the fastest index: neighbours read one row's parts
+  const int slot = (int)(blockIdx.x / (2u * p.c.kv)), hz = (int)(blockIdx.x - slot * (2u * p.c.kv));
+  const int z = hz >= p.c.kv, h = z ? hz - p.c.kv : hz;
+  int entry = slot / blocks_per_seq, nth = slot % blocks_per_seq;
+  if (p.b.cu) {
+    const int sh = p.c.block_shift;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    for (int i = tid; i < p.b.m; i += 128) {
+      const int a = (p.b.cu[i] >> sh) + 2 * i, b = (p.b.cu[i + 1] >> sh) + 2 * (i + 1);
+      if (slot >= a && slot < b) {
+        found[0] = i;
+        found[1] = slot - a;
+      }
+    }
+    __syncthreads();
+    entry = found[0];
+    nth = found[1];
+    if (entry < 0) return;
+  }
   Touched<T> o;
-  if (!touched<T, D>(p, blockIdx.x / blocks_per_seq, blockIdx.x % blocks_per_seq, blockIdx.y, blockIdx.z, tid == 0, o))
-    return;
+  if (!find_rows<T>(p, entry, nth, h, z, tid == 0, o)) return;
   const int n = o.to - o.from;
   uint4 w[P];
 #pragma unroll
@@ -105,6 +142,7 @@ __global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, i
       }
     }
   }
+  if (!__syncthreads_and(find_page<T, D>(p.c, tid == 0, o))) return;
   const float s0 = o.from > o.b0 ? *o.scale : 0.0f;
   float a = 0.0f;
 #pragma unroll
@@ -159,12 +197,9 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
   const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   Touched<T> o;
-  if (!touched<T, D>(p, (int)(unit / blocks_per_seq), (int)(unit % blocks_per_seq), blockIdx.y, blockIdx.z, lane == 0,
-                     o))
+  if (!find_rows<T>(p, (int)(unit / blocks_per_seq), (int)(unit % blocks_per_seq), blockIdx.y, blockIdx.z, lane == 0, o))
     return;
   const int b0 = o.b0, from = o.from, to = o.to;
-  int8_t *dst = o.dst;
-  float *sp = o.scale;
 
   constexpr int E = D / 32;  // elements of a row per lane
   float a = 0.0f;
@@ -176,6 +211,9 @@ __global__ void __launch_bounds__(128) append_kernel(const AppendArgs p, int blo
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if (!__all_sync(0xffffffffu, find_page<T, D>(p.c, lane == 0, o))) return;
+  int8_t *dst = o.dst;
+  float *sp = o.scale;
   const float s0 = from > b0 ? *sp : 0.0f;
   const float want = a >= kTiny ? __fmul_rn(a, 1.0f / 127.0f) : 0.0f;
   const float sc = fmaxf(s0, want);
@@ -207,8 +245,12 @@ static int launch_append(const AppendArgs &a, cudaStream_t st) {
       return ((uintptr_t)p | (uintptr_t)(row * (int64_t)sizeof(T)) | (uintptr_t)(head * (int64_t)sizeof(T))) % 16 == 0;
     };
     const int vec = fits(a.k, a.k_row, a.k_head) && fits(a.v, a.v_row, a.v_head);
-    dim3 grid((unsigned)((int64_t)a.b.m * per), a.c.kv, 2);
-    append_block_kernel<T, D><<<grid, 128, 0, st>>>(a, per, vec);
+    const int64_t slots = a.b.cu ? (a.b.total >> a.c.block_shift) + 2 * a.b.m + 1 : (int64_t)a.b.m * per;
+    if (slots * 2 * a.c.kv > INT32_MAX) {
+      set_error("kv8_append: too many rows");
+      return kErrInvalid;
+    }
+    append_block_kernel<T, D><<<(unsigned)(slots * 2 * a.c.kv), 128, 0, st>>>(a, per, vec);
   } else {
     dim3 grid((unsigned)ceil_div((int64_t)a.b.m * per, 4), a.c.kv, 2);
     append_kernel<T, D><<<grid, 128, 0, st>>>(a, per);
@@ -230,19 +272,29 @@ int append(const AppendArgs &a, cudaStream_t st) {
 
 // ---- reading back --------------------------------------------------------------
 
-// One warp per token, all its heads (their loads are independent):
-// code * scale; tokens without a page read as 0.
+// One warp per packed row, all its heads (their loads are independent):
+// code * scale; tokens without a page read as 0.  With cu the lanes look for
+// the row's entry.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   const Layer &c = p.c;
   const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int i = (int)(unit / p.b.n), j = (int)(unit % p.b.n);
-  if (i >= p.b.m) return;
+  if (unit >= p.b.total) return;
+  int i = -1;
+  if (p.b.cu) {
+    for (int e = lane; e < p.b.m; e += 32)
+      if (unit >= p.b.cu[e] && unit < p.b.cu[e + 1]) i = e;
+    i = __reduce_max_sync(0xffffffffu, i);
+  } else {
+    i = (int)((uint32_t)unit / (uint32_t)p.b.n);
+  }
+  if (i < 0) return;
   int64_t row0;
   int count;
   p.b.rows(i, row0, count);
-  if (j >= count) return;
+  const int j = (int)(unit - row0);
+  if (j < 0 || j >= count) return;
   const int s = p.b.seq(i, c.n_seqs);
   if (s < 0 && lane == 0) atomicOr(c.status, kBadSeq);
   const int tok = s < 0 ? -1 : seq_length(c, s) - count + j;
@@ -276,7 +328,7 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
 
 template <typename T, int D>
 static int launch_rows(const RowsArgs &a, cudaStream_t st) {
-  rows_kernel<T, D><<<(unsigned)ceil_div((int64_t)a.b.m * a.b.n, 4), 128, 0, st>>>(a);
+  rows_kernel<T, D><<<(unsigned)ceil_div(a.b.total, 4), 128, 0, st>>>(a);
   SC_CUDA(cudaGetLastError());
   note_launch();
   return kOk;
