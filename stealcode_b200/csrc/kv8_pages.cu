@@ -16,6 +16,11 @@
 // word; while a bit is set, reserve, fork, compact and append do nothing, so
 // a step queued behind a failed one cannot write over a page.  release and
 // slide always run: giving pages back is how a caller recovers.
+//
+// Measured: reserving 256 prompts in a pool of 87 k pages 15 us (a chain of
+// cluster barriers and table loads), release and slide 4.6 us each; forking
+// 256 hypotheses over 24 layers 131 us, of them 117 for 684 MB of page copies
+// (5.9 TB/s); moving half of 24 layers' pages 302 us for 1.7 GB (5.7 TB/s).
 #include <atomic>
 
 #include <cooperative_groups.h>
