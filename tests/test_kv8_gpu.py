@@ -388,6 +388,63 @@ def test_attend_split_over_a_long_past(torch, dtype, n):
     del a
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_long_chunks_without_alignment(torch, dtype, d):
+    """Rows and results at odd element offsets, through the many-row kernel and the block-wise append; one
+    sequence long enough that its items are split."""
+    rng = np.random.default_rng(d)
+    c, r = make(torch, d=d, kv=2, page=48, block=16, n_seqs=2, max_pages=40, n_pages=90)
+    for s, n in ((0, 90), (1, 1500)):
+        assert r.reserve([s], [n])
+        c.reserve(ids(torch, [n]), seqs=ids(torch, [s]))
+        flat = torch.tensor(rng.standard_normal(n * 5 * d + 3), dtype=torch.float32, device="cuda").to(dt(torch, dtype))
+        kv = flat[3:].view(n, 5, d)
+        put(torch, c, r, [s], [n], [kv[:, 1:3], kv[:, 3:5]])
+    same(torch, c, r)
+    flat = torch.tensor(rng.standard_normal(180 * 7 * d + 1), dtype=torch.float32, device="cuda").to(dt(torch, dtype))
+    q = flat[1:].view(180, 7, d)[:, 1:]
+    out = torch.zeros(180 * 8 * d + 1, dtype=q.dtype, device="cuda")[1:].view(180, 8, d)
+    check_attend(torch, c, r, [1, 0], [90, 90], 6, dtype, rng, q=q, out=out[:, 1:7])
+    assert not out[:, 0].any() and not out[:, 7].any()
+    # scores turned round, and all alike
+    for scale in (-0.3, 0.0):
+        w = torch.zeros(180, 6, d, dtype=q.dtype, device="cuda")
+        w.copy_(q)
+        a, la = c.attend(0, w, seqs=ids(torch, [1, 0]), n=90, scale=scale, return_lse=True)
+        b, lb = c.attend(0, w * -1 if scale else w * 0, seqs=ids(torch, [1, 0]), n=90, scale=-scale or 1.0, return_lse=True)
+        assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_offsets_beyond_32_bits(torch, n):
+    """Pages whose codes start beyond 2^32 bytes: the same bits as from a small pool."""
+    from stealcode_b200 import KvCache8
+
+    pages, used = 70000, 12
+    big = KvCache8(1, pages, 8, 128, 2, 8, page=64, block=32)  # 64 KB a page
+    small = KvCache8(1, used, 8, 128, 2, 8, page=64, block=32)
+    big.refs[:pages - used] = 1  # in use by others
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(500, 8, 128, generator=g, device="cuda") for _ in range(2))
+    q = torch.randn(2 * n, 16, 128, generator=g, device="cuda")
+    got = []
+    for c in (big, small):
+        c.reserve(ids(torch, [330, 170]))
+        c.append(0, k, v, cu=ids(torch, [0, 330, 500]), n=330)
+        out = c.attend(0, q, n=n, max_len=330)
+        rows = c.rows(0, cu=ids(torch, [0, 330, 500]), n=330, total=500)
+        c.release(ids(torch, [0]))
+        c.fork(ids(torch, [1]), ids(torch, [0]))
+        out2 = c.attend(0, q, n=n, max_len=330)
+        c.check()
+        got.append((out, out2) + rows)
+    assert int(big.table.max()) == int(small.table.max()) + pages - used
+    assert int(big.table[1, 0]) * 65536 > 2 ** 32
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_attend_in_a_cuda_graph(torch):
     rng = np.random.default_rng(16)
     c, r = make(torch, d=128, kv=2, page=32, block=16, n_seqs=2, max_pages=8)
