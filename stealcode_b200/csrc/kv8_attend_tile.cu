@@ -525,28 +525,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         soft_sync();
         if (sh.last) {
           __threadfence();
-          // a thread joins 16 elements of a row
-          for (int u = tid; u < nr * (D / 16); u += 512) {
-            const int rr = u / (D / 16), d0 = u % (D / 16) * 16;
-            float top = -INFINITY, sum = 0.0f, acc[16];
-            for (int k = 0; k < pc.parts; k++)
-              top = fmaxf(top, __ldcg(g.parts + (int64_t)part_slot(pc.c0, k) * kPart + kTileRows * D + rr));
+          // a thread joins 8 elements of a row, in one pass: a part's loads
+          // wait for nothing before them, four parts are on their way
+          for (int u = tid; u < nr * (D / 8); u += 512) {
+            const int rr = u / (D / 8), d0 = u % (D / 8) * 8;
+            float top = -INFINITY, sum = 0.0f, acc[8];
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[e] = 0.0f;
-#pragma unroll 2
+            for (int e = 0; e < 8; e++) acc[e] = 0.0f;
+#pragma unroll 4
             for (int k = 0; k < pc.parts; k++) {
               const float *y = g.parts + (int64_t)part_slot(pc.c0, k) * kPart;
               const float pm = __ldcg(y + kTileRows * D + rr), pl = __ldcg(y + kTileRows * D + kTileRows + rr);
-              const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - top);
-              sum += f * pl;
+              const float4 va = __ldcg((const float4 *)(y + rr * D + d0)), vb = __ldcg((const float4 *)(y + rr * D + d0) + 1);
+              const float now = fmaxf(top, pm);
+              const float old = now == -INFINITY ? 1.0f : exp2_approx(top - now);
+              const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - now);
+              top = now;
+              sum = sum * old + f * pl;
+              const float v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const float4 v = __ldcg((const float4 *)(y + rr * D + d0) + e);
-                acc[4 * e] += f * v.x;
-                acc[4 * e + 1] += f * v.y;
-                acc[4 * e + 2] += f * v.z;
-                acc[4 * e + 3] += f * v.w;
-              }
+              for (int e = 0; e < 8; e++) acc[e] = acc[e] * old + f * v[e];
             }
             int j2, h2;
             en.row(g, rr, j2, h2);
@@ -554,8 +552,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kTileShift);
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
-            for (int e = 0; e < 16; e++) acc[e] *= inv;
-            store_row<T, 16>(dst, acc, vec_o);
+            for (int e = 0; e < 8; e++) acc[e] *= inv;
+            store_row<T, 8>(dst, acc, vec_o);
             if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
           }
@@ -819,7 +817,19 @@ static int launch_tile(const AttendArgs &a, int sm_count, cudaStream_t st) {
   g.magic = (uint32_t)((2097152 + g.group - 1) / g.group);
   g.per_seq = (int)ceil_div((int64_t)a.b.n * g.group, kTileRows);
   g.entries = a.b.m * g.per_seq;
+  // Where there are fewer units than blocks could take: a share of u tiles of an
+  // item of n costs u tiles' time and n / u parts to join, each by its rows, so
+  // u near sqrt(n rows / 256) (4 heads of 128, bf16; shares of 2, 4, 8, 16: 256
+  // rows over 2048 tokens 53, 48, 55, 79 us, over 8192 121, 83, 72, 86; 64 rows
+  // over 8192 42, 35, 38, 53).  Items of a few tiles are not split: 256 rows
+  // over 512 tokens 26 us whole, 36 in shares of 2.
+  int64_t keys = a.max_len;
+  if (a.window > 0 && (int64_t)a.window + a.b.n + a.sinks + 2 * kTileKeys < keys)
+    keys = (int64_t)a.window + a.b.n + a.sinks + 2 * kTileKeys;
+  const int64_t tiles = ceil_div(keys, kTileKeys), all = (int64_t)a.b.n * g.group, rows = all < kTileRows ? all : kTileRows;
   g.min_share = 2;
+  while ((int64_t)g.min_share * g.min_share * kTileRows < tiles * rows && g.min_share < 64) g.min_share++;
+  if (tiles + kTileOver <= 8) g.min_share = (int)tiles + kTileOver;
   g.count = (int32_t *)a.ws;
   g.parts = (float *)((char *)a.ws + kMaxBlocks * 4);
   const bool vq = ((uintptr_t)a.q & 15) == 0 && a.q_row * sizeof(T) % 16 == 0 && a.q_head * sizeof(T) % 16 == 0;
