@@ -22,7 +22,6 @@ the host; failures that only the device sees (too few free pages) are read with
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from ctypes import c_int32, c_int64, c_void_p
 
@@ -48,8 +47,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
-
-_NO_STREAM = contextlib.nullcontext()
 
 
 class _Cache(ctypes.Structure):
@@ -161,21 +158,22 @@ class KvCache8:
         return _Batch(self._ids(seqs, "seqs"), self._ids(cu, "cu"), m, n, total)
 
     def _rows_in(self, t, heads: int, name: str):
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.head_dim or t.dtype not in _DTYPES or \
-                t.device != self.device or (t.stride(2) != 1 and t.numel()):
+        """The strides of a checked row tensor."""
+        shape, strides = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self.head_dim or t.dtype not in _DTYPES or \
+                t.device != self.device or (strides[2] != 1 and t.numel()):
             raise ValueError(f"{name} has to be [rows, {heads}, {self.head_dim}] f32, f16 or bf16 on {self.device}, "
                              "dense in its last dimension")
+        return strides
 
     # ---- rows ---------------------------------------------------------------------
 
     def append(self, layer: int, k, v, *, seqs=None, cu=None, n=None, stream=None) -> None:
         """Quantise k, v [rows, n_kv_heads, head_dim] into the sequences' last tokens."""
-        self._rows_in(k, self.n_kv_heads, "k")
-        self._rows_in(v, self.n_kv_heads, "v")
+        ks, vs = self._rows_in(k, self.n_kv_heads, "k"), self._rows_in(v, self.n_kv_heads, "v")
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError("k and v differ in type or shape")
         b = self._batch(seqs, cu, n, k.shape[0])
-        ks, vs = k.stride(), v.stride()
         rc = lib.sc_kv8_append(self._p, layer, ctypes.byref(b), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
                                _DTYPES[k.dtype], self._stream(stream))
         if rc:
@@ -188,10 +186,14 @@ class KvCache8:
         if dtype not in _DTYPES:
             raise ValueError("dtype has to be f32, f16 or bf16")
         st = self._stream(stream)
-        # allocations belong to the stream that uses them
-        with _NO_STREAM if stream is None else torch.cuda.stream(stream):
-            k = self.k_scale.new_empty((b.total, self.n_kv_heads, self.head_dim), dtype=dtype)
+        shape = (b.total, self.n_kv_heads, self.head_dim)
+        if stream is None:
+            k = self.k_scale.new_empty(shape, dtype=dtype)
             v = torch.empty_like(k)
+        else:  # allocations belong to the stream that uses them
+            with torch.cuda.stream(stream):
+                k = self.k_scale.new_empty(shape, dtype=dtype)
+                v = torch.empty_like(k)
         rc = lib.sc_kv8_rows(self._p, layer, ctypes.byref(b), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], st)
         if rc:
             check(rc)
@@ -207,20 +209,29 @@ class KvCache8:
         ``max_len``: no sequence is longer (sizes the launch).  ``scale``: head_dim ** -0.5 if None."""
         if q.dim() != 3 or q.shape[1] < 1:
             raise ValueError("q has to be [rows, n_heads, head_dim]")
-        heads = q.shape[1]
-        self._rows_in(q, heads, "q")
-        b = self._batch(seqs, cu, n, q.shape[0])
+        rows, heads = q.shape[:2]
+        qs = self._rows_in(q, heads, "q")
+        b = self._batch(seqs, cu, n, rows)
         st = self._stream(stream)
         if out is not None:
-            self._rows_in(out, heads, "out")
+            os_ = self._rows_in(out, heads, "out")
             if out.dtype != q.dtype or out.shape != q.shape:
                 raise ValueError("out has to have q's type and shape")
-        with _NO_STREAM if stream is None else torch.cuda.stream(stream):
+        lse = None
+        if stream is None:
             if out is None:
                 out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            lse = self.k_scale.new_empty((q.shape[0], heads)) if return_lse else None
-        ws = self._workspace("attend", st, stream, lib.sc_kv8_attend_workspace_bytes)
-        qs, os_ = q.stride(), out.stride()
+                os_ = out.stride()
+            if return_lse:
+                lse = self.k_scale.new_empty((rows, heads))
+        else:  # allocations belong to the stream that uses them
+            with torch.cuda.stream(stream):
+                if out is None:
+                    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                    os_ = out.stride()
+                if return_lse:
+                    lse = self.k_scale.new_empty((rows, heads))
+        ws = self._ws.get(("attend", st)) or self._workspace("attend", st, stream, lib.sc_kv8_attend_workspace_bytes)
         rc = lib.sc_kv8_attend(self._p, layer, ctypes.byref(b), q.data_ptr(), qs[0], qs[1], heads,
                                self.head_dim ** -0.5 if scale is None else scale, window, sinks, max_len,
                                out.data_ptr(), os_[0], os_[1], lse.data_ptr() if return_lse else None,
