@@ -18,7 +18,8 @@ sequences 0, 1, ...
 
 Everything runs on the current torch stream (or ``stream``) without a copy to
 the host; failures that only the device sees (too few free pages) are read with
-``check()``.
+``check()``.  Calls can be captured in a CUDA graph once the same kind of call
+has run on that stream: the first one makes the stream's workspace.
 """
 from __future__ import annotations
 
@@ -131,6 +132,9 @@ class KvCache8:
         """(address, bytes) of this stream's workspace, zeroed when it is made."""
         ws = self._ws.get((kind, st))
         if ws is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("kv8: make one such call on this stream before a graph capture (the workspace "
+                                   "would belong to the graph)")
             n = need()
             check(min(n, 0))
             with torch.cuda.stream(torch.cuda.current_stream() if stream is None else stream):

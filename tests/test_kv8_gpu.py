@@ -472,6 +472,17 @@ def test_attend_in_a_cuda_graph(torch):
         assert torch.equal(out, c.attend(0, q, n=1))
     check_attend(torch, c, r, [0, 1], [1, 1], 4, "f32", rng, q=q)
     del g
+    # a capture on a stream that has no workspace yet is refused
+    h, other = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    x = torch.zeros(4, device="cuda")
+    with torch.cuda.graph(h, stream=other):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="before a graph capture"):
+            c.attend(0, q, n=1)
+    h.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 1).all())
+    del h
 
 
 # ---- pages ---------------------------------------------------------------------------
