@@ -13,10 +13,12 @@
 // f16 (exact for f16 and, down to 2^-38 of the row's largest value, bf16
 // inputs), or as hi + lo in two f16 for f32 inputs (22 bits); products and
 // sums are f32.  With x = scale * log2(e) * q.k:
-//   e = 2^(x - m),  w = e * vs * 2^8,  l += e,  O += w * code(v)
-// where m bounds x + log2(vs) up to 2^7, so w stays inside f16 (or hi + lo
-// of two f16 for f32) whatever the value scales are.  m only grows when a
-// score passes it by more than 7: the accumulators are rarely rescaled.
+//   e = 2^(x - r),  w = e * 2^(log2(vs) + c),  l += e,  O += w * code(v)
+// where r bounds x up to 2^64 and r - c + 8 bounds x + log2(vs) up to 2^7: l
+// has its own reference, so neither it nor w (f16, or hi + lo of two f16 for
+// f32) leaves its range whatever the value scales are.  r and c change when a
+// score passes one of the bounds, so the accumulators are rarely rescaled;
+// they are whole numbers, so their factors are powers of two.
 //
 // What bounds it: the codes' bytes, 2 * head_dim a token and kv head.  A warp
 // takes 16 tokens at a time with 16-byte loads straight into registers, and
@@ -43,8 +45,10 @@ namespace kv8 {
 constexpr int kStepTile = 64;    // tokens per tile: 16 for each warp
 constexpr int kStepThreads = 128;
 constexpr int kStepOver = 1;
-constexpr float kShift = 256.0f;  // 2^8
-constexpr float kSlack = 7.0f;
+constexpr float kShift = 8.0f;     // a row's largest weight is 2^7 .. 2^8 when the references are set,
+constexpr float kWide = 15.0f;     // and below 2^15 as long as they are kept
+constexpr float kWideSum = 64.0f;  // log2 of a term of l, likewise
+constexpr float kNothing = -1e30f; // r of a row that has seen nothing
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
@@ -80,7 +84,7 @@ struct StepShared {
   static constexpr int kLd = D + 2;
   uint2 q[2][NT][D / 16][32];       // hi and lo fragments of q
   float qf[kRows];                  // score factor of each row
-  float m[4][kRows], l[4][kRows];
+  float r[4][kRows], u[4][kRows], l[4][kRows];  // of each warp; u = c - r: O is in units of 2^u
   float o[4][kRows][kLd];
   ShareScratch share;
   int last;
@@ -230,14 +234,15 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       }
 
     float o[KS][NT][4];
-    float m[NT][2], l[NT][2];
+    float ref[NT][2], off[NT][2], l[NT][2];  // r, c, l
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
       for (int i = 0; i < KS; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) o[i][n][e] = 0.0f;
-      m[n][0] = m[n][1] = -INFINITY;
+      ref[n][0] = ref[n][1] = kNothing;
+      off[n][0] = off[n][1] = kShift;
       l[n][0] = l[n][1] = 0.0f;
     }
 
@@ -299,6 +304,11 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       const float lv = log2_approx(vf);
       const bool all = cur.tok + 15 <= en.p_lo &&
                        (p.window <= 0 || cur.tok > en.p_hi - p.window || cur.tok + 15 < p.sinks);
+      float most[NT][2];  // no score above these: the references stand
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) most[n][u] = ref[n][u] + fminf(kWideSum, kWide - (off[n][u] + lv));
       bool grow = false;
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -311,20 +321,22 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
             v = see ? v : -INFINITY;
           }
           s[n][e] = v;
-          grow |= v + lv > m[n][e & 1] + kSlack;
+          grow |= v > most[n][e & 1];
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            float top = fmaxf(s[n][u], s[n][u + 2]) + lv;
+            float top = fmaxf(s[n][u], s[n][u + 2]);
 #pragma unroll
             for (int q = 4; q < 32; q <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
-            const float now = fmaxf(m[n][u], top);
-            const float f = now == -INFINITY ? 1.0f : exp2_approx(m[n][u] - now);
-            m[n][u] = now;
-            l[n][u] *= f;
+            const float r0 = ref[n][u], r1 = fmaxf(r0, ceilf(top));
+            const float b0 = r0 - off[n][u], b1 = fmaxf(b0, ceilf(top + lv) - kShift);  // -u
+            const float f = exp2_approx(b0 - b1);
+            ref[n][u] = r1;
+            off[n][u] = r1 - b1;
+            l[n][u] *= exp2_approx(r0 - r1);
 #pragma unroll
             for (int i = 0; i < KS; i++) {
               o[i][n][u] *= f;
@@ -332,17 +344,17 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
             }
           }
       }
-      const float wf = vf * kShift;
       uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float w[4];
+        float w[4], wf[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) wf[u] = exp2_approx(fminf(off[n][u] + lv, 126.0f));
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float mm = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
-          const float v = exp2_approx(s[n][e] - mm);
+          const float v = exp2_approx(s[n][e] - ref[n][e & 1]);
           l[n][e & 1] += v;
-          w[e] = v * wf;
+          w[e] = v * wf[e & 1];
         }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -385,7 +397,8 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
         for (int q = 4; q < 32; q <<= 1) v += __shfl_xor_sync(0xffffffffu, v, q);
         const int r = n * 8 + 2 * ti + u;
         if (gi == 0) {
-          sh.m[warp][r] = m[n][u];
+          sh.r[warp][r] = ref[n][u];
+          sh.u[warp][r] = off[n][u] - ref[n][u];
           sh.l[warp][r] = v;
         }
 #pragma unroll
@@ -394,18 +407,18 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       }
     __syncthreads();
     const int slot = pc.starts ? 2 * (int)blockIdx.x + 1 : 2 * (int)blockIdx.x;
-    constexpr int kPart = ROWS * (D + 2);
+    constexpr int kPart = ROWS * (D + 3);
     float *part = g.parts + (int64_t)slot * kPart;
     // a warp takes a row, a lane D / 32 of its elements
     constexpr int E = D / 32;
-    auto store = [&](int r, float top, float sum, const float (&acc)[E]) {
+    auto store = [&](int r, float top, float unit, float sum, const float (&acc)[E]) {
       int j, hq;
       en.row(g, r, j, hq);
       hq += pc.head * g.group;
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kShift);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, back = exp2_approx(-(top + unit));
       T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
 #pragma unroll
-      for (int e = 0; e < E; e++) dst[e * 32 + lane] = from_f32<T>(acc[e] * inv);
+      for (int e = 0; e < E; e++) dst[e * 32 + lane] = from_f32<T>(acc[e] * inv * back);
       if (p.lse && lane == 0)
         p.lse[(en.row0 + j) * p.n_heads + hq] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
     };
@@ -413,27 +426,30 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
     for (int i = 0; i < ROWS / 4; i++) {
       const int r = warp + 4 * i;
       if (r >= nr) break;
-      float top = -INFINITY, sum = 0.0f, acc[E];
+      float top = kNothing, unit = -kNothing, sum = 0.0f, acc[E];
 #pragma unroll
-      for (int w = 0; w < 4; w++) top = fmaxf(top, sh.m[w][r]);
+      for (int w = 0; w < 4; w++) {
+        top = fmaxf(top, sh.r[w][r]);
+        unit = fminf(unit, sh.u[w][r]);
+      }
 #pragma unroll
       for (int e = 0; e < E; e++) acc[e] = 0.0f;
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        const float f = sh.m[w][r] == -INFINITY ? (sh.l[w][r] != sh.l[w][r] ? sh.l[w][r] : 0.0f)
-                                                : exp2_approx(sh.m[w][r] - top);
-        sum += f * sh.l[w][r];
+        const float f = exp2_approx(unit - sh.u[w][r]);
+        sum += exp2_approx(sh.r[w][r] - top) * sh.l[w][r];
 #pragma unroll
         for (int e = 0; e < E; e++) acc[e] += f * sh.o[w][r][e * 32 + lane];
       }
       if (pc.whole) {
-        store(r, top, sum, acc);
+        store(r, top, unit, sum, acc);
       } else {
 #pragma unroll
         for (int e = 0; e < E; e++) part[r * D + e * 32 + lane] = acc[e];
         if (lane == 0) {
           part[ROWS * D + r] = top;
           part[ROWS * D + ROWS + r] = sum;
+          part[ROWS * D + 2 * ROWS + r] = unit;
         }
       }
     }
@@ -449,24 +465,30 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
       if (sh.last) {
         __threadfence();
         for (int r = warp; r < nr; r += 4) {
-          float top = -INFINITY;
-          for (int k = lane; k < pc.parts; k += 32)
-            top = fmaxf(top, __ldcg(g.parts + (int64_t)part_slot(pc.c0, k) * kPart + ROWS * D + r));
+          float top = kNothing, unit = -kNothing;
+          for (int k = lane; k < pc.parts; k += 32) {
+            const float *q = g.parts + (int64_t)part_slot(pc.c0, k) * kPart + ROWS * D + r;
+            top = fmaxf(top, __ldcg(q));
+            unit = fminf(unit, __ldcg(q + 2 * ROWS));
+          }
 #pragma unroll
-          for (int q = 16; q > 0; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+          for (int q = 16; q > 0; q >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+            unit = fminf(unit, __shfl_xor_sync(0xffffffffu, unit, q));
+          }
           float sum = 0.0f, acc[E];
 #pragma unroll
           for (int e = 0; e < E; e++) acc[e] = 0.0f;
 #pragma unroll 4
           for (int k = 0; k < pc.parts; k++) {
             const float *q = g.parts + (int64_t)part_slot(pc.c0, k) * kPart;
-            const float pm = __ldcg(q + ROWS * D + r), pl = __ldcg(q + ROWS * D + ROWS + r);
-            const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - top);
-            sum += f * pl;
+            const float pr = __ldcg(q + ROWS * D + r), pl = __ldcg(q + ROWS * D + ROWS + r);
+            const float f = exp2_approx(unit - __ldcg(q + ROWS * D + 2 * ROWS + r));
+            sum += exp2_approx(pr - top) * pl;
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] += f * __ldcg(q + r * D + e * 32 + lane);
           }
-          store(r, top, sum, acc);
+          store(r, top, unit, sum, acc);
         }
       }
     }
@@ -475,7 +497,7 @@ __global__ void __launch_bounds__(kStepThreads, NT == 1 ? 4 : 3)
 }
 
 size_t attend_ws_bytes(int sm_count) {
-  const size_t step = (size_t)sm_count * 4 * 2 * 16 * 130 * 4;
+  const size_t step = (size_t)sm_count * 4 * 2 * 16 * 131 * 4;
   const size_t tile = tile_ws_bytes(sm_count);
   return kMaxBlocks * 4 + (step > tile ? step : tile);
 }

@@ -1,7 +1,9 @@
 // kv8_attend_tile.cu -- attention over the paged 8-bit cache for many query
 // rows per kv head (prompts, long chunks), on the tensor cores' own memory.
-// Formulas and numerics are kv8_attend.cu's; the parts of split items and the
-// sharing-out are kv8_work.cuh's.
+// Formulas and numerics are kv8_attend.cu's, with one reference for a row's sum
+// and its output (e = 2^(x - m), w = e * vs * gain * 2^8, m bounds
+// x + log2(vs * gain)) and two gains for the value scales; the parts of split
+// items and the sharing-out are kv8_work.cuh's.
 //
 // A block takes 256 rows (token, query head of the group) as two tiles of 128
 // and walks the keys 128 at a time:
@@ -54,6 +56,27 @@ constexpr int kTileOver = 3;
 constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
 constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
 
+// The value scales vs that a piece computes with are vs * gain, so that a
+// row's sum l of 2^(x - m), where m bounds x + log2(vs * gain), stays inside
+// f32 with bits to spare.  Gain 2^8: exponents from -80 (vs = 2^72) to 98.6
+// (the smallest scale, 1e-30 / 127), to which up to 7 (m's slack) and the
+// tokens' number are added.  A piece of work that meets a larger vs goes on
+// with gain 2^-40 (up to vs = 2^121, the largest): its old results are scaled
+// by 2^-48, and scales below 2^-60 are held against 2^-60 then, so what a row
+// draws from them loses bits and at last vanishes beside those of 2^72.
+constexpr float kGain = 256.0f, kGainLog2 = 8.0f, kBigGain = 0x1p-40f, kBigScale = 0x1p72f;
+constexpr float kToBig = 0x1p-48f, kFromBig = 0x1p48f, kToBigLog2 = -48.0f;
+constexpr float kLeastLog2 = -100.0f;  // of vs * gain
+constexpr float kBigSum = 0x1p60f;     // sums above it are not scaled by 2^48
+
+// l * 2^d for a sum l, f = 2^d: with scales far apart 2^d can underflow
+// where the product does not.
+__device__ __forceinline__ float scale_sum(float l, float d, float f) {
+  if (d > -100.0f) return l * f;
+  const float h = exp2_approx(0.5f * d);
+  return l * h * h;
+}
+
 template <int D, bool SPLIT>
 struct TileCfg {
   static constexpr int kStages = SPLIT && D == 128 ? 1 : 2;
@@ -66,17 +89,25 @@ struct TileCfg {
 struct TileShared {  // after the operands
   uint64_t q_full[2], s_full[2], p_full[2], pv_done[2];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  // a key tile's 16-token groups: score factor ks, log2(vs), weight factor
-  // vs * 2^8, and whether the group has a page; four tiles deep, so a slot is
-  // written again only after both softmaxes have read it
-  float kf[4][8], lv[4][8], wf[4][8];
-  uint32_t live[4][4];  // two bits from each converter warp
+  // a key tile's 16-token groups: score factor ks, log2(vs * gain), weight
+  // factor vs * gain * 2^8 (slots 0-3 for kGain, 4-7 for kBigGain), and whether
+  // the group has a page (bit 8: the piece has come to a scale above kBigScale,
+  // so its gain is kBigGain); four tiles deep, so a slot is written again only
+  // after both softmaxes have gone through the next tile too
+  float kf[8][8], lv[8][8], wf[8][8];
+  uint32_t live[4][4];  // two bits from each converter warp, and bit 8
   float top[2][2][2][128];  // [tile parity][row tile][half][row]: largest score, and once a piece the sums
+  float sum[2][2][128];     // [row tile][half][row] sums where the gain turns to kBigGain
   ShareScratch share;
   uint32_t tmem;
   int last;
   volatile int started;  // pieces the softmax warps have begun
 };
+
+// Which groups of a tile have a page (bits 0-7), and whether its gain is kBigGain.
+__device__ __forceinline__ uint32_t live_word(const TileShared &sh, int slot) {
+  return sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
+}
 
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -292,6 +323,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       hq += pc.head * g.group;
       const int pos = mine ? en.first + j : -1;
       float m = -INFINITY, l = 0.0f;
+      bool big = false;  // the gain at the piece's end
       if (tid == 0) sh.started = sh.started + 1;
       if (on && nt > 0) {
         // the pair of warps loads its 32 rows, 16 each
@@ -319,10 +351,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (ok) ok = mbar_wait(&sh.s_full[q], (uint32_t)ns & 1u);
           __syncwarp();
           tc_fence_after();
-          const int slot = (nk + x) & 3;
-          const uint32_t live = sh.live[slot][0] | sh.live[slot][1] | sh.live[slot][2] | sh.live[slot][3];
+          const uint32_t live = live_word(sh, (nk + x) & 3);
+          const int slot = ((nk + x) & 3) + (int)(live >> 8) * 4;
+          if (live > 0xffu) sh.sum[q][half][row] = l;
           const int t0 = en.tile(pc.t0 + x) * kTileKeys;
-          const bool all = live == 0xffu && t0 + kTileKeys - 1 <= p_lo &&
+          const bool all = (live & 0xffu) == 0xffu && t0 + kTileKeys - 1 <= p_lo &&
                            (p.window <= 0 || t0 > p_hi - p.window || t0 + kTileKeys - 1 < p.sinks);
           if (!all) {  // -inf over what the row does not see, in tensor memory
 #pragma unroll 1
@@ -364,12 +397,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           sh.top[x & 1][q][half][row] = top;
           pair_sync(pair);
           top = fmaxf(top, sh.top[x & 1][q][half ^ 1][row]);
-          const bool grow = top > m + (x ? kTileSlack : 0.0f);
-          if (__any_sync(0xffffffffu, grow)) {
+          bool grow = top > m + (x ? kTileSlack : 0.0f);
+          if (__any_sync(0xffffffffu, grow || live > 0xffu)) {
+            float f = 1.0f;  // factor of the output accumulator
+            if (live > 0xffu && x && live_word(sh, (nk + x - 1) & 3) <= 0xffu) {  // the gain turns
+              if (fmaxf(l, sh.sum[q][half ^ 1][row]) <= kBigSum) {  // the same O under a smaller bound
+                l *= kFromBig;
+                m += kToBigLog2;
+              } else {
+                f = kToBig;
+              }
+              grow = top > m + kTileSlack;
+            }
             const float now = grow ? top : m;
-            const float f = grow ? exp2_approx(m - now) : 1.0f;
+            const float fl = grow ? exp2_approx(m - now) : 1.0f;
+            if (grow) l = scale_sum(l, m - now, fl);
             m = now;
-            l *= f;
+            f *= fl;
             if (x) {  // every product into O before this tile's has completed (see the MMA warp)
 #pragma unroll 1
               for (int i = half * (D / 64); i < (half + 1) * (D / 64); i++) {
@@ -420,6 +464,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           }
           l += lo_of(l2) + hi_of(l2);
+          big = live > 0xffu;
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -442,7 +487,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_fence_after();
         }
         const int pr = q * 128 + row;  // row of the item
-        const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / (l * kTileShift)) : 1.0f;
+        const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        const float unit = pc.whole ? 1.0f / (kTileShift * (big ? kBigGain : kGain)) : 1.0f;
         T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
         // A whole item's rows go through the queries' shared memory (their
         // last product has completed), 16-byte pieces swizzled by the row, so
@@ -466,7 +512,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int t = 0; t < 4; t++) {  // 8 consecutive elements
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(o[8 * (e / 2) + 2 * t + (e & 1)]) * inv;
+            for (int e = 0; e < 8; e++) v[e] = __uint_as_float(o[8 * (e / 2) + 2 * t + (e & 1)]) * inv * unit;
             const int d0 = (i >> 1) * 64 + t * 16 + (i & 1) * 8;
             if (staged) {
               constexpr int W = 16 / sizeof(T);
@@ -510,7 +556,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (p.lse) p.lse[(en.row0 + j) * p.n_heads + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
           } else {
             part[kTileRows * D + pr] = m;
-            part[kTileRows * D + kTileRows + pr] = l;
+            part[kTileRows * D + kTileRows + pr] = big ? -l : l;  // the sign tells of the gain
           }
         }
         tc_fence_before();  // O has been read before the next piece's first product overwrites it
@@ -532,6 +578,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int u = tid; u < nr * (D / 8); u += 512) {
             const int rr = u / (D / 8), d0 = u % (D / 8) * 8;
             float top = -INFINITY, sum = 0.0f, acc[8];
+            bool any_big = false;
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = 0.0f;
 #pragma unroll 4
@@ -542,19 +589,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               const float now = fmaxf(top, pm);
               const float old = now == -INFINITY ? 1.0f : exp2_approx(top - now);
               const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - now);
+              sum = (now == -INFINITY ? sum : scale_sum(sum, top - now, old)) +
+                    (pm == -INFINITY ? f : scale_sum(fabsf(pl), pm - now, f));
               top = now;
-              sum = sum * old + f * pl;
+              const bool was = any_big;
+              any_big |= signbit(pl);
+              const float fo = any_big != was ? old * kToBig : old, fv = any_big && !signbit(pl) ? f * kToBig : f;
               const float v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-              for (int e = 0; e < 8; e++) acc[e] = acc[e] * old + f * v[e];
+              for (int e = 0; e < 8; e++) acc[e] = acc[e] * fo + fv * v[e];
             }
             int j2, h2;
             en.row(g, rr, j2, h2);
             h2 += pc.head * g.group;
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kTileShift);
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float unit = 1.0f / (kTileShift * (any_big ? kBigGain : kGain));
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) acc[e] *= inv;
+            for (int e = 0; e < 8; e++) acc[e] = acc[e] * inv * unit;
             store_row<T, 8>(dst, acc, vec_o);
             if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -592,6 +644,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       };
       uint4 kr[4][HF], vr[4][HF];
       float ks = 1.0f, vs = 1.0f;  // lanes 0, 1: the scales of the warp's groups
+      uint32_t large = 0;
       auto load_k = [&](int x, const int (&pid)[2]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -660,12 +713,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         const int slot = nk & 3;
         if (lane < 2) {
-          const float v = vs > 0.0f ? vs : 1.0f;
-          sh.kf[slot][2 * w + lane] = ks > 0.0f ? ks : 1.0f;  // a scale of 0 has codes of 0
-          sh.lv[slot][2 * w + lane] = log2_approx(v);
-          sh.wf[slot][2 * w + lane] = v * kTileShift;
+          // a scale of 0 has codes of 0: any factor does that keeps the weights inside f16
+          const float v = vs > 0.0f ? vs : 1.0f / kGain;
+          const float lv = log2_approx(v) + kGainLog2;
+          const int gr = 2 * w + lane;
+          sh.kf[slot][gr] = sh.kf[slot + 4][gr] = ks > 0.0f ? ks : 1.0f;
+          sh.lv[slot][gr] = lv;
+          sh.lv[slot + 4][gr] = fmaxf(lv + kToBigLog2, kLeastLog2);
+          sh.wf[slot][gr] = v * (kTileShift * kGain);
+          sh.wf[slot + 4][gr] = v * (kTileShift * kBigGain);
         }
-        if (lane == 0) sh.live[slot][w] = ((pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u)) << (2 * w);
+        if (__any_sync(0xffffffffu, lane < 2 && vs > kBigScale)) large = 0x100u;
+        if (lane == 0) sh.live[slot][w] = ((pid[0] >= 0 ? 1u : 0u) | (pid[1] >= 0 ? 2u : 0u)) << (2 * w) | large;
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[st]);

@@ -202,8 +202,7 @@ __device__ __forceinline__ float log2_approx(float x) {
   return y;
 }
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kMaxBlocks = 4096;  // counters at the start of the workspace
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;constexpr int kMaxBlocks = 4096;  // counters at the start of the workspace
 
 }  // namespace kv8
 }  // namespace sc
