@@ -478,6 +478,7 @@ int sc_rnnt_destroy(sc_rnnt_decoder *r);
 #define SC_KV8_BAD_SEQUENCE 4u  /* sequence id outside the cache or named twice, or a negative count */
 #define SC_KV8_BAD_PAGE 8u      /* page id outside the cache, or an append without a reserved page */
 #define SC_KV8_WAIT_TIMEOUT 16u /* a bounded device-side wait gave up */
+#define SC_KV8_BAD_ROWS 32u     /* an entry of cu with more than n rows, fewer than 0, or rows outside the packed ones */
 
 #define SC_DTYPE_F32 0
 #define SC_DTYPE_F16 1
@@ -495,7 +496,10 @@ typedef struct {
 /* The rows of a call: m sequences, row r of the i-th (sequence seqs[i], or i
  * when seqs is NULL) at packed row cu[i] + r, cu[i + 1] - cu[i] rows of it
  * (cu NULL: n rows each), at most n; `total` packed rows in all.  seqs, cu:
- * device arrays.  No sequence is named twice. */
+ * device arrays.  No sequence is named twice.  Packed rows that no entry has
+ * (before cu[0], from cu[m] on) are neither read nor written.  An entry with
+ * more than n rows, fewer than 0 or rows outside the packed ones has none and
+ * sets SC_KV8_BAD_ROWS. */
 typedef struct {
   const int32_t *seqs, *cu;
   int64_t m, n, total;

@@ -26,6 +26,7 @@ enum : unsigned {
   kBadSeq = SC_KV8_BAD_SEQUENCE,
   kBadPage = SC_KV8_BAD_PAGE,
   kWaitTimeout = SC_KV8_WAIT_TIMEOUT,
+  kBadRows = SC_KV8_BAD_ROWS,
 };
 
 // One layer of a cache (pointers already at that layer).
@@ -49,20 +50,21 @@ struct Batch {
   int m, n;
   int64_t total;
 
-  // start >= 0, start + count <= total and count <= n whatever cu holds, so
-  // no value of cu leads outside the packed tensors.
-  __device__ __forceinline__ void rows(int i, int64_t &start, int &count) const {
+  // False for an entry that cu describes wrongly (from a row before the first,
+  // to one past the total, fewer than 0 rows or more than n): it has no rows
+  // then, so no value of cu leads outside the packed tensors, and none makes
+  // some of an entry's rows stand for other tokens.
+  __device__ __forceinline__ bool rows(int i, int64_t &start, int &count) const {
     if (!cu) {
       start = (int64_t)i * n;
       count = n;
-      return;
+      return true;
     }
     const int64_t a = cu[i], b = cu[i + 1];
-    start = a < 0 ? 0 : a;
-    int64_t c = b - start;
-    if (c > total - start) c = total - start;
-    if (c > n) c = n;
-    count = c < 0 ? 0 : (int)c;
+    const bool ok = a >= 0 && b >= a && b <= total && b - a <= n;
+    start = ok ? a : 0;
+    count = ok ? (int)(b - a) : 0;
+    return ok;
   }
   // The sequence of entry i, or -1 (outside the cache).
   __device__ __forceinline__ int seq(int i, int n_seqs) const {

@@ -61,7 +61,10 @@ __device__ __forceinline__ bool find_rows(const AppendArgs &p, int i, int bi, in
   }
   int64_t row0;
   int count;
-  p.b.rows(i, row0, count);
+  if (!p.b.rows(i, row0, count)) {
+    if (tell) atomicOr(c.status, kBadRows);
+    return false;
+  }
   const int len = seq_length(c, o.s), first = len - count;
   // rows before position 0 (more new rows than the sequence holds) are left out
   const int lo = first < 0 ? 0 : first;
@@ -122,6 +125,9 @@ __global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, i
         found[0] = i;
         found[1] = slot - a;
       }
+      int64_t row0;
+      int count;  // block 0 sees every entry, also those that take no slot
+      if (blockIdx.x == 0 && !p.b.rows(i, row0, count)) atomicOr(p.c.status, kBadRows);
     }
     __syncthreads();
     entry = found[0];
@@ -291,8 +297,13 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   if (unit >= p.b.total) return;
   int i = -1;
   if (p.b.cu) {
-    for (int e = lane; e < p.b.m; e += 32)
-      if (unit >= p.b.cu[e] && unit < p.b.cu[e + 1]) i = e;
+    for (int e = lane; e < p.b.m; e += 32) {
+      int64_t start;
+      int count;
+      const bool ok = p.b.rows(e, start, count);
+      if (unit >= start && unit < start + count) i = e;
+      if (unit == 0 && !ok) atomicOr(c.status, kBadRows);
+    }
     i = __reduce_max_sync(0xffffffffu, i);
   } else {
     i = (int)((uint32_t)unit / (uint32_t)p.b.n);

@@ -36,6 +36,7 @@ struct Entry {
   int j0, h0;       // row r0's token (from row0) and query head
   int p_lo, p_hi;   // positions of the first and the last row
   int a, b, c;
+  unsigned bad;     // status bits of what is wrong with entry i
   __device__ __forceinline__ int tiles() const { return a + c - b; }
   __device__ __forceinline__ int steps() const { return max(1, tiles()); }  // an item without keys has a result too
   __device__ __forceinline__ int tile(int x) const { return x < a ? x : b + x - a; }
@@ -53,7 +54,7 @@ template <int ROWS, int TILE>
 __device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g, int e, Entry &o) {
   o.i = (int)((uint32_t)e / (uint32_t)g.per_seq);
   int count;
-  p.b.rows(o.i, o.row0, count);
+  o.bad = p.b.rows(o.i, o.row0, count) ? 0u : (unsigned)kBadRows;
   o.r0 = (e - o.i * g.per_seq) * ROWS;
   const int rows = count * g.group;
   if (o.r0 >= rows) return false;
@@ -104,9 +105,13 @@ __device__ bool find_share(const AttendArgs &p, const WorkGrid &g, ShareScratch 
   const int per = (g.entries + THREADS - 1) / THREADS;
   const int e0 = min(tid * per, g.entries), e1 = min(e0 + per, g.entries);
   int64_t mine = 0;
+  unsigned bad = 0;
   Entry en;
-  for (int e = e0; e < e1; e++)
+  for (int e = e0; e < e1; e++) {
     if (get_entry<ROWS, TILE>(p, g, e, en)) mine += (int64_t)(OVER + en.steps()) * p.c.kv;
+    bad |= en.bad;
+  }
+  if (bad && blockIdx.x == 0) atomicOr(p.c.status, bad);
   int64_t x = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {

@@ -13,7 +13,8 @@ scale per block of tokens and kv head, in pages that sequences can share
 ``append``, ``attend`` and ``rows`` work on the last tokens of each sequence.
 Their rows are packed: ``n`` rows for each sequence, or, with ``cu`` (int32
 CUDA tensor [m + 1]), rows ``cu[i] .. cu[i + 1]`` for the i-th, at most ``n``
-each.  ``seqs`` (int32 CUDA tensor [m]) names the sequences; None means
+each.  Rows before ``cu[0]`` and from ``cu[m]`` on belong to no sequence: they
+are not touched, and hold anything in an output that the call allocates.  ``seqs`` (int32 CUDA tensor [m]) names the sequences; None means
 sequences 0, 1, ...
 
 Everything runs on the current torch stream (or ``stream``) without a copy to
@@ -31,7 +32,7 @@ import torch
 from . import _lib
 from ._lib import SC_ERR_ALLOC, SC_ERR_INVALID, SC_ERR_TIMEOUT, ScError, check, lib
 
-POOL_FULL, TABLE_FULL, BAD_SEQUENCE, BAD_PAGE, WAIT_TIMEOUT = 1, 2, 4, 8, 16
+POOL_FULL, TABLE_FULL, BAD_SEQUENCE, BAD_PAGE, WAIT_TIMEOUT, BAD_ROWS = 1, 2, 4, 8, 16, 32
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _FAILURES = (
@@ -39,6 +40,7 @@ _FAILURES = (
     (TABLE_FULL, SC_ERR_ALLOC, "a sequence is longer than its table row"),
     (BAD_SEQUENCE, SC_ERR_INVALID, "a sequence id outside the cache or named twice, or a negative count"),
     (BAD_PAGE, SC_ERR_INVALID, "a page id outside the cache, or an append without a reserved page"),
+    (BAD_ROWS, SC_ERR_INVALID, "cu gives an entry more than n rows, fewer than 0, or rows outside the packed ones"),
     (WAIT_TIMEOUT, SC_ERR_TIMEOUT, "a bounded device-side wait gave up"),
 )
 
