@@ -525,7 +525,8 @@ int sc_kv8_rows(const sc_kv8_cache *c, int64_t layer, const sc_kv8_batch *b,
  * at position p sees the tokens t <= p that still have a page and, with
  * window > 0, t > p - window or t < sinks.  out = softmax(scale * q k) v in
  * q's dtype, lse (f32 [total][n_heads], may be NULL) the log of the sum of
- * exponentials; a query that sees nothing gets 0 and -inf.  max_len: no
+ * exponentials; a query that sees nothing, or whose sequence id lies outside
+ * the cache (SC_KV8_BAD_SEQUENCE), gets 0 and -inf.  max_len: no
  * sequence is longer (<= 0: unknown); a hint that sizes the launch.
  * workspace: sc_kv8_attend_workspace_bytes (of the current device), 256-byte
  * aligned, zeroed once before its first use; calls that may overlap need one

@@ -60,6 +60,7 @@ __device__ __forceinline__ bool get_entry(const AttendArgs &p, const WorkGrid &g
   if (o.r0 >= rows) return false;
   o.r1 = min(rows, o.r0 + ROWS);
   o.s = p.b.seq(o.i, p.c.n_seqs);
+  if (o.s < 0) o.bad = kBadSeq;
   const int len = o.s < 0 ? 0 : seq_length(p.c, o.s);
   o.first = len - count;
   o.j0 = (int)((uint32_t)o.r0 / (uint32_t)g.group);

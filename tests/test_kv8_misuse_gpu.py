@@ -82,3 +82,20 @@ def test_packed_rows_of_no_entry_are_not_touched(torch):
     r.append(0, [0, 1], [h[0][3:40], h[0][40:60]], [h[1][3:40], h[1][40:60]])
     c.check()
     same(torch, c, r)
+
+
+@pytest.mark.parametrize("n", [1, 60])
+def test_attend_reports_sequences_outside_the_cache(torch, n):
+    rng = np.random.default_rng(12)
+    c, r = make(torch, d=64, kv=1, max_pages=12)
+    fill(torch, c, r, [0], [70], rng)
+    q = torch.tensor(rng.standard_normal((3 * n, 2, 64)), dtype=torch.float32, device="cuda")
+    for seqs in ([7, 0, -1], [0, 1, 4]):
+        out, lse = c.attend(0, q, seqs=ids(torch, seqs), n=n, return_lse=True)
+        for i, s in enumerate(seqs):
+            a = slice(i * n, (i + 1) * n)
+            assert bool(out[a].any()) == (s == 0) and bool(torch.isneginf(lse[a]).all()) == (s != 0)
+        fails(torch, c, "sequence id")
+    # an entry without rows names nothing
+    c.attend(0, q[:1], seqs=ids(torch, [0, 99]), cu=ids(torch, [0, 1, 1]), n=1)
+    c.check()
