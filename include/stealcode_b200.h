@@ -472,7 +472,10 @@ int sc_rnnt_destroy(sc_rnnt_decoder *r);
  * Failures that only the device can see set bits of the status word.  A
  * reserve, fork or compact that fails changes nothing; while a bit is set,
  * reserve, fork, compact and append do nothing (release and slide run), until
- * the caller writes 0. */
+ * the caller writes 0.  An append that fails itself has written some of its
+ * rows and not others: they are undefined, in all sequences of its batch, until
+ * they are appended again; nothing else changes (older rows of a block that the
+ * call touched may have been rounded to the block's new scale). */
 #define SC_KV8_POOL_FULL 1u     /* too few free pages */
 #define SC_KV8_TABLE_FULL 2u    /* a sequence past max_pages */
 #define SC_KV8_BAD_SEQUENCE 4u  /* sequence id outside the cache or named twice, or a negative count */

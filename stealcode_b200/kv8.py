@@ -175,7 +175,10 @@ class KvCache8:
     # ---- rows ---------------------------------------------------------------------
 
     def append(self, layer: int, k, v, *, seqs=None, cu=None, n=None, stream=None) -> None:
-        """Quantise k, v [rows, n_kv_heads, head_dim] into the sequences' last tokens."""
+        """Quantise k, v [rows, n_kv_heads, head_dim] into the sequences' last tokens.
+
+        An append that fails on the device (see ``check``) leaves these tokens undefined until they are
+        appended again."""
         ks, vs = self._rows_in(k, self.n_kv_heads, "k"), self._rows_in(v, self.n_kv_heads, "v")
         if k.dtype != v.dtype or k.shape != v.shape:
             raise ValueError("k and v differ in type or shape")

@@ -99,3 +99,30 @@ def test_attend_reports_sequences_outside_the_cache(torch, n):
     # an entry without rows names nothing
     c.attend(0, q[:1], seqs=ids(torch, [0, 99]), cu=ids(torch, [0, 1, 1]), n=1)
     c.check()
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_an_append_that_fails_is_repeated(torch, n):
+    """One sequence of the batch has no pages for its rows: the call fails, leaves every other sequence alone, and
+    the same rows appended again once there are pages give what an append without the failure gives."""
+    rng = np.random.default_rng(n)
+    c, r = make(torch, d=64, kv=2, page=16, block=16, n_seqs=5, max_pages=10, n_pages=50)
+    fill(torch, c, r, [0, 1, 2, 3], [21, 5, 50, 9], rng)
+    assert r.reserve([0, 3], [n, n])
+    c.reserve(ids(torch, [n, n]), seqs=ids(torch, [0, 3]))
+    x = [torch.tensor(rng.standard_normal((3 * n, 2, 64)) * 3, dtype=torch.float32, device="cuda") for _ in range(2)]
+    h = [y.cpu().numpy() for y in x]
+    keep = c.k.clone(), c.k_scale.clone(), c.v.clone(), c.v_scale.clone()
+    c.length[1] += 16 * 8  # tokens that no page was reserved for
+    c.append(0, *x, seqs=ids(torch, [0, 1, 3]), n=n)
+    fails(torch, c, "page id")
+    pages = c.table[2][c.table[2] >= 0].long()
+    for t, old in zip((c.k, c.k_scale, c.v, c.v_scale), keep):
+        assert torch.equal(t[:, pages].nan_to_num(3.0), old[:, pages].nan_to_num(3.0))
+    c.length[1] = 5
+    assert r.reserve([1], [n])
+    c.reserve(ids(torch, [n]), seqs=ids(torch, [1]))
+    c.append(0, *x, seqs=ids(torch, [0, 1, 3]), n=n)
+    r.append(0, [0, 1, 3], *[[y[i * n:(i + 1) * n] for i in range(3)] for y in h])
+    c.check()
+    same(torch, c, r)
