@@ -115,13 +115,26 @@ class KvCache8:
                          self.n_seqs, self.max_pages, self.n_kv_heads, self.head_dim, self.page, self.block)
         self._p = ctypes.addressof(self._c)
         self._ws = {}  # (kind, stream) -> workspace: calls on two streams never share one
+        self._named = set()  # streams that calls have named
 
     # ---- arguments ----------------------------------------------------------------
 
-    def _stream(self, stream) -> int:
+    def _stream(self, stream, *used) -> int:
+        """The call's stream.  A stream that the call names reads the cache and the tensors ``used``: their
+        memory is not given out again before that work is done."""
         if _current_device() != self._index:
             raise ValueError(f"the cache lives on {self.device}, the current device is {_current_device()}")
-        return _raw_stream(self._index) if stream is None else stream.cuda_stream
+        if stream is None:
+            return _raw_stream(self._index)
+        st = stream.cuda_stream
+        if st not in self._named:
+            for t in (self.k, self.v, self.k_scale, self.v_scale, self.table, self.length, self.refs, self.status):
+                t.record_stream(stream)
+            self._named.add(st)
+        for t in used:
+            if t is not None:
+                t.record_stream(stream)
+        return st
 
     def _ids(self, t, name: str) -> int:
         if t is None:
@@ -184,7 +197,7 @@ class KvCache8:
             raise ValueError("k and v differ in type or shape")
         b = self._batch(seqs, cu, n, k.shape[0])
         rc = lib.sc_kv8_append(self._p, layer, ctypes.byref(b), k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
-                               _DTYPES[k.dtype], self._stream(stream))
+                               _DTYPES[k.dtype], self._stream(stream, k, v, seqs, cu))
         if rc:
             check(rc)
 
@@ -194,7 +207,7 @@ class KvCache8:
         b = self._batch(seqs, cu, n, total)
         if dtype not in _DTYPES:
             raise ValueError("dtype has to be f32, f16 or bf16")
-        st = self._stream(stream)
+        st = self._stream(stream, seqs, cu)
         shape = (b.total, self.n_kv_heads, self.head_dim)
         if stream is None:
             k = self.k_scale.new_empty(shape, dtype=dtype)
@@ -221,11 +234,13 @@ class KvCache8:
         rows, heads = q.shape[:2]
         qs = self._rows_in(q, heads, "q")
         b = self._batch(seqs, cu, n, rows)
-        st = self._stream(stream)
+        st = self._stream(stream, q, seqs, cu)
         if out is not None:
             os_ = self._rows_in(out, heads, "out")
             if out.dtype != q.dtype or out.shape != q.shape:
                 raise ValueError("out has to have q's type and shape")
+            if stream is not None:
+                out.record_stream(stream)
         lse = None
         if stream is None:
             if out is None:
@@ -259,9 +274,10 @@ class KvCache8:
         p = self._ids(counts, "counts")
         if seqs is not None and seqs.shape != counts.shape:
             raise ValueError("seqs and counts differ in length")
-        st = self._stream(stream)
+        s = self._ids(seqs, "seqs")
+        st = self._stream(stream, counts, seqs)
         ws = self._page_ws(st, stream)
-        check(lib.sc_kv8_reserve(self._p, self._ids(seqs, "seqs"), p, counts.shape[0], ws[0], ws[1], st))
+        check(lib.sc_kv8_reserve(self._p, s, p, counts.shape[0], ws[0], ws[1], st))
 
     def fork(self, parents, children, *, stream=None) -> None:
         """children[i] becomes a copy of parents[i] (int32 CUDA tensors [m]; all pairs at once, so a parent
@@ -270,19 +286,19 @@ class KvCache8:
         a, b = self._ids(parents, "parents"), self._ids(children, "children")
         if parents.shape != children.shape:
             raise ValueError("parents and children differ in length")
-        st = self._stream(stream)
+        st = self._stream(stream, parents, children)
         ws = self._page_ws(st, stream)
         check(lib.sc_kv8_fork(self._p, a, b, parents.shape[0], ws[0], ws[1], st))
 
     def release(self, seqs=None, *, stream=None) -> None:
         """Give back the sequences' pages; their lengths become 0.  None: all sequences."""
         m = self.n_seqs if seqs is None else seqs.shape[0]
-        check(lib.sc_kv8_release(self._p, self._ids(seqs, "seqs"), m, self._stream(stream)))
+        check(lib.sc_kv8_release(self._p, self._ids(seqs, "seqs"), m, self._stream(stream, seqs)))
 
     def slide(self, window: int, sinks: int = 0, *, seqs=None, stream=None) -> None:
         """Give back the pages that no later query can see under this window and these sinks."""
         m = self.n_seqs if seqs is None else seqs.shape[0]
-        check(lib.sc_kv8_slide(self._p, self._ids(seqs, "seqs"), m, window, sinks, self._stream(stream)))
+        check(lib.sc_kv8_slide(self._p, self._ids(seqs, "seqs"), m, window, sinks, self._stream(stream, seqs)))
 
     def compact(self, *, stream=None) -> None:
         """Move the pages in use to the lowest ids; the tables follow."""
