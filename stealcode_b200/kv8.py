@@ -147,12 +147,12 @@ class KvCache8:
         """(address, bytes) of this stream's workspace, zeroed when it is made."""
         ws = self._ws.get((kind, st))
         if ws is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("kv8: make one such call on this stream before a graph capture (the workspace "
-                                   "would belong to the graph)")
-            n = need()
-            check(min(n, 0))
             with torch.cuda.stream(torch.cuda.current_stream() if stream is None else stream):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("kv8: make one such call on this stream before a graph capture (the workspace "
+                                       "would belong to the graph)")
+                n = need()
+                check(min(n, 0))
                 buf = torch.zeros(n, dtype=torch.uint8, device=self.device)
             ws = self._ws[(kind, st)] = (buf.data_ptr(), n, buf)
         return ws

@@ -1,6 +1,5 @@
 """GPU tests of the paged 8-bit cache's calls on a stream that is named in the
-call:
-their inputs and the cache outlive the work."""
+call: their inputs outlive the work, and a capture on that stream is seen."""
 import numpy as np
 import pytest
 
@@ -91,3 +90,28 @@ def test_a_cache_outlives_its_work_on_another_stream(torch):
         torch.cuda.synchronize()
         del hold
     assert torch.equal(got[0], got[1]) and got[0].any()
+
+
+def test_a_capture_on_the_named_stream_is_refused(torch):
+    """The stream of the call captures, the current one does not: no workspace is made inside the graph."""
+    rng = np.random.default_rng(3)
+    c, r = make(torch, d=64, kv=1)
+    fill(torch, c, r, [0], [9], rng)
+    q = torch.zeros(4, 2, 64, device="cuda")
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    x = torch.zeros(4, device="cuda")
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    refused = False
+    with torch.cuda.graph(g, stream=side, capture_error_mode="relaxed"):
+        x.add_(1)
+        with torch.cuda.stream(other):
+            try:
+                c.attend(0, q, n=1, out=out, stream=side)
+            except RuntimeError as e:
+                refused = "before a graph capture" in str(e)
+    g.replay()
+    torch.cuda.synchronize()
+    assert refused and bool((x == 1).all())
+    del g
