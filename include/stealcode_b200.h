@@ -533,7 +533,7 @@ int sc_kv8_rows(const sc_kv8_cache *c, int64_t layer, const sc_kv8_batch *b,
  * sequence is longer (<= 0: unknown); a hint that sizes the launch.
  * workspace: sc_kv8_attend_workspace_bytes (of the current device), 256-byte
  * aligned, zeroed once before its first use; calls that may overlap need one
- * each. */
+ * each (a graph's replay uses the one that its call was captured with). */
 int64_t sc_kv8_attend_workspace_bytes(void);
 int sc_kv8_attend(const sc_kv8_cache *c, int64_t layer,
                   const sc_kv8_batch *b, const void *q, int64_t q_row,

@@ -20,7 +20,10 @@ sequences 0, 1, ...
 Everything runs on the current torch stream (or ``stream``) without a copy to
 the host; failures that only the device sees (too few free pages) are read with
 ``check()``.  Calls can be captured in a CUDA graph once the same kind of call
-has run on that stream: the first one makes the stream's workspace.
+has run on that stream: the first one makes the stream's workspace.  A graph
+keeps the workspace of the stream that it was captured on: wherever it is
+replayed, the replay has to be ordered against every other call and replay that
+uses that workspace (capture on a stream of its own for graphs that overlap).
 """
 from __future__ import annotations
 
@@ -114,7 +117,7 @@ class KvCache8:
                          length.data_ptr(), refs.data_ptr(), self.status.data_ptr(), self.n_layers, self.n_pages,
                          self.n_seqs, self.max_pages, self.n_kv_heads, self.head_dim, self.page, self.block)
         self._p = ctypes.addressof(self._c)
-        self._ws = {}  # (kind, stream) -> workspace: calls on two streams never share one
+        self._ws = {}  # (kind, stream) -> workspace: calls on two streams share none, replays see the module's text
         self._named = set()  # streams that calls have named
 
     # ---- arguments ----------------------------------------------------------------
