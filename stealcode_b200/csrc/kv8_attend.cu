@@ -10,9 +10,10 @@
 //
 // Numerics.  The codes are whole numbers and exact in f16.  A row of q is
 // scaled by a power of two to a largest magnitude in [2^13, 2^14) and held in
-// f16 (exact for f16 and, down to 2^-38 of the row's largest value, bf16
-// inputs), or as hi + lo in two f16 for f32 inputs (22 bits); products and
-// sums are f32.  With x = scale * log2(e) * q.k:
+// f16, or as hi + lo in two f16 for f32 inputs (22 bits): an element of a f16
+// or bf16 row is exact where it is above 2^-27 (f16) or 2^-30 (bf16: 8 bits) of
+// the row's largest, and no element of any type is off by more than 2^-38 of
+// that (an f16's smallest step, 2^-24, halved).  Products and sums are f32.  With x = scale * log2(e) * q.k:
 //   e = 2^(x - r),  w = e * 2^(log2(vs) + c),  l += e,  O += w * code(v)
 // where r bounds x up to 2^64 and r - c + 8 bounds x + log2(vs) up to 2^7: l
 // has its own reference, so neither it nor w (f16, or hi + lo of two f16 for

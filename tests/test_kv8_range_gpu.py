@@ -28,8 +28,9 @@ def torch():
     return _t
 
 
-def check_weighted(torch, c, r, s, n, heads, dtype, q, window=0, sinks=0):
-    """attend's results for the last n tokens of s against 64 bits, each element within what its own terms allow."""
+def check_weighted(torch, c, r, s, n, heads, dtype, q, window=0, sinks=0, floor=0.0):
+    """attend's results for the last n tokens of s against 64 bits, each element within what its own terms allow.
+    floor: the error of an element of q, of the row's largest."""
     scale = r.d ** -0.5
     out, lse = c.attend(0, q, seqs=ids(torch, [s]), n=n, window=window, sinks=sinks, return_lse=True)
     c.check()
@@ -54,11 +55,14 @@ def check_weighted(torch, c, r, s, n, heads, dtype, q, window=0, sinks=0):
         p = e / e.sum(1, keepdims=True)
         ref, rl = p @ vh, m[:, 0] + np.log(e.sum(1))
         size = np.where(see, np.abs(qh[:, h]) @ np.abs(kh).T, 0).max(1) * scale
-        ds = size * (2.0 ** -22 + 2 * r.d * u) + 2.0 ** -22 * (size + 256)
+        reach = np.abs(qh[:, h]).max(1) * np.where(see, np.abs(kh).sum(1)[None], 0).max(1) * scale
+        ds = floor * reach + size * (2.0 ** -22 + 2 * r.d * u) + 2.0 ** -22 * (size + 256)
         tol = (p @ np.abs(vh)) * (np.exp(2 * ds) - 1 + wt + 2.0 ** -18)[:, None] + \
             length * 2.0 ** -32 * 127 * (p * sh).max(1)[:, None]
         err = np.abs(got[:, h] - ref)
-        limit = tol + rnd * np.abs(ref) + 1e-44
+        # half a step of the type, which is fixed below its normal numbers
+        fi = torch.finfo(q.dtype)
+        limit = tol + np.maximum(rnd * np.abs(ref), fi.tiny * fi.eps / 2)
         bad = ~(err <= limit)
         assert not bad.any(), (h, int(bad.sum()), float(got[:, h][bad][0]), float(ref[bad][0]), float(limit[bad][0]))
         assert np.all(np.abs(z[:, h] - rl) <= ds + 2.0 ** -18 + 2.0 ** -21 * np.abs(rl))
@@ -137,3 +141,55 @@ def test_tiny_values_of_a_long_past(torch, rows):
     n, d = 40000, 64
     c, r = filled(torch, rng.standard_normal((n, 1, d)), rng.uniform(-1, 1, (n, 1, d)) * 2.0 ** -99, block=32)
     check_weighted(torch, c, r, 1, rows, 4, "f32", queries(torch, rng, rows, 4, d, "f32", 0.3))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 60])
+def test_growing_keys_and_scales_far_apart(torch, rows, dtype):
+    """Scores that grow along the past (the references move in every tile) over value blocks between 2^-20 and 2^12,
+    for small, ordinary and large queries."""
+    rng = np.random.default_rng(rows)
+    n, d = 700, 128
+    x = rng.standard_normal((n, 1, d))
+    grow = np.linspace(0.01, 4, n)[:, None, None]
+    e = rng.integers(-20, 10, -(-n // 16)).repeat(16)[:n]
+    c, r = filled(torch, x * grow, x * np.exp2(e)[:, None, None])
+    for size in (1e-4, 1.0, 20.0):
+        check_weighted(torch, c, r, 1, rows, 4, dtype, queries(torch, rng, rows, 4, d, dtype, size))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [300, 2500])
+def test_rows_that_are_not_finite_spoil_themselves_only(torch, n, dtype):
+    """In the many-row kernel, whole items and split ones."""
+    rng = np.random.default_rng(n)
+    rows, d = 60, 64
+    c, r = filled(torch, rng.standard_normal((n, 1, d)), rng.standard_normal((n, 1, d)))
+    q = queries(torch, rng, rows, 4, d, dtype, 1.5)
+    clean, lse = c.attend(0, q, seqs=ids(torch, [1]), n=rows, return_lse=True)
+    bad = [(0, 0, float("nan")), (31, 2, float("inf")), (32, 0, -float("inf")), (59, 3, float("nan"))]
+    q2, keep = q.clone(), torch.ones(rows, 4, dtype=torch.bool)
+    for t, h, x in bad:
+        q2[t, h, (t * 7) % d] = x
+        keep[t, h] = False
+    got, lse2 = c.attend(0, q2, seqs=ids(torch, [1]), n=rows, return_lse=True)
+    assert torch.isnan(got[~keep]).all() and not torch.isfinite(lse2[~keep]).any()
+    assert torch.equal(got[keep], clean[keep]) and torch.equal(lse2[keep], lse[keep])
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 60])
+def test_queries_of_many_sizes_in_one_row(torch, rows, dtype):
+    """A row is held relative to its largest element: each element is off by at most 2^-38 of that.  Rows with an
+    element near 60000 that no key has any of, beside subnormal f16 numbers and ordinary ones that decide."""
+    rng = np.random.default_rng(rows)
+    n, d = 300, 64
+    keys = rng.standard_normal((n, 1, d)) * 3000.0
+    keys[..., :2] = 0.0
+    c, r = filled(torch, keys, rng.standard_normal((n, 1, d)))
+    q = np.exp2(rng.uniform(-24, -10, (rows, 4, d))) * rng.choice([-1, 1], (rows, 4, d))
+    q[..., 0] = rng.uniform(30000, 65000, (rows, 4))
+    q[: rows // 2, :, 0] = 2.0  # some rows without it
+    q = torch.tensor(q, dtype=torch.float32, device="cuda").to(dt(torch, dtype))
+    check_weighted(torch, c, r, 1, rows, 4, dtype, q, floor=2.0 ** -38)
