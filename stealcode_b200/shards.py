@@ -40,16 +40,19 @@ class StreamShards:
 
     step(s) posts this rank's heartbeat for step s, waits up to `timeout_s`
     for the others' and returns (lo, hi, taken_over): this rank's span for
-    step s and the streams in it that another rank held at step s - 1.  A
-    rank that misses a step's heartbeat is dropped for good; every survivor
-    sees the same set (a late rank that posts after the others gave up on
-    it is still dropped: it finds itself missing from the step's member list
-    and must stop)."""
+    step s and the streams in it that another rank held at step s - 1.  The
+    first step waits up to `start_timeout_s`: ranks start at different times
+    (processes, contexts, weights).  A rank that misses a step's heartbeat is
+    dropped for good; every survivor sees the same set (a late rank that posts
+    after the others gave up on it is still dropped: it finds itself missing
+    from the step's member list and must stop)."""
 
     def __init__(self, store, rank: int, world: int, global_streams: int, timeout_s: float = 5.0,
-                 prefix: str = "shards"):
+                 prefix: str = "shards", start_timeout_s: float = 60.0):
         self.store, self.rank, self.world = store, rank, world
         self.global_streams, self.timeout_s, self.prefix = global_streams, timeout_s, prefix
+        self.start_timeout_s = max(timeout_s, start_timeout_s)
+        self.started = False
         self.live: List[int] = list(range(world))
         self.spans = plan(global_streams, self.live)
 
@@ -58,7 +61,9 @@ class StreamShards:
 
     def step(self, step: int) -> Tuple[int, int, List[int]]:
         self.store.set(self._key(step, self.rank), "1")
-        deadline = time.monotonic() + self.timeout_s
+        window = self.timeout_s if self.started else self.start_timeout_s
+        self.started = True
+        deadline = time.monotonic() + window
         seen = {self.rank}
         while len(seen) < len(self.live):
             for r in self.live:
@@ -73,7 +78,7 @@ class StreamShards:
         leader = min(seen)
         if self.rank == leader:
             self.store.compare_set(members_key, "", ",".join(str(r) for r in sorted(seen)))
-        self.store.wait([members_key], _timedelta(self.timeout_s * 4))
+        self.store.wait([members_key], _timedelta(window * 4))
         members = [int(v) for v in self.store.get(members_key).decode().split(",")]
         if self.rank not in members:
             raise RuntimeError(f"rank {self.rank} was dropped at step {step}")
