@@ -22,7 +22,12 @@ namespace sc {
 namespace kv8 {
 
 constexpr float kTiny = 1e-30f;
-constexpr int kStepRows = 8;  // up to this many rows a sequence, a warp takes a block
+// Up to this many rows a sequence, a warp takes a block.  A warp and a block of
+// threads, 64 sequences, 8 heads of 128, f32: 4 rows 6.8 and 9.5 us, 8 rows 8.3
+// and 10.3, 12 rows 10.3 and 10.3, 64 rows 23 and 18.8; 4 sequences: 8 rows 8.3
+// and 7, 64 rows 16.5 and 7.  (256 sequences gain from warps up to 32 rows: 27
+// and 41.)
+constexpr int kStepRows = 8;
 
 __device__ __forceinline__ float finite_mag(float x) {
   const float a = fabsf(x);
@@ -97,12 +102,12 @@ __device__ __forceinline__ bool find_page(const Layer &c, bool tell, Touched<T> 
 // Many rows: one block of 128 threads holds the new rows of one touched block
 // in registers (64 rows of 128 f32 are 64 registers a thread), so they are
 // read once, with every load in flight at the same time.
-template <typename T, int D>
 //
 // Uneven rows (cu): entry i's touched blocks take the slots from
 // cu[i] / block + 2 i, which leaves room for one more block at either end, so
 // the grid has total / block + 2 m slots instead of m times the longest
 // entry's; a block of threads finds its entry with one load a thread.
+template <typename T, int D>
 __global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, int blocks_per_seq, int vec) {
   constexpr int N = 16 / sizeof(T);  // elements of a load
   constexpr int C = D / N;           // loads of a row

@@ -65,20 +65,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-// Bytes (0, 1) or (2, 3) of a word of codes, each with its top bit flipped
-// (code + 128), as two f16: 0x6400 | u is 1024 + u.
-__device__ __forceinline__ uint32_t two_f16(uint32_t w, uint32_t sel) {
-  const uint32_t u = __byte_perm(w, 0x64646464u, sel);
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-constexpr uint32_t kLow = 0x4140, kHigh = 0x4342;
-
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 template <int D, int NT>
 struct StepShared {
   static constexpr int kRows = 8 * NT;
@@ -549,8 +535,10 @@ static int step(const AttendArgs &a, int sm_count, cudaStream_t st) {
 
 int attend(const AttendArgs &a, int sm_count, cudaStream_t st) {
   if (a.b.m == 0 || a.b.n == 0 || a.b.total == 0) return kOk;
-  // Above 32 rows per kv head the tensor-memory kernel: 8 sequences of 4000
-  // tokens, bf16, 32 rows: 50 us here, 56 there; 48 rows: 65 and 58.
+  // Above 32 rows per kv head the tensor-memory kernel.  8 sequences of 4000
+  // tokens, 8 kv heads, 32 rows, here and there: bf16 heads of 128 50 and 56 us,
+  // of 64 41 and 45, f32 61 and 73, 43 and 57; 48 rows: 66 and 58, 51 and 45, 80
+  // and 74, 55 and 57.  Of 500 tokens: 32 rows 23 and 23 (bf16), 25 and 27 (f32).
   if ((int64_t)a.b.n * (a.n_heads / a.c.kv) > 32) return attend_tile(a, sm_count, st);
   if (a.dtype == SC_DTYPE_F32) return step<float>(a, sm_count, st);
   if (a.dtype == SC_DTYPE_F16) return step<__half>(a, sm_count, st);

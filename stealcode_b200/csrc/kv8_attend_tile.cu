@@ -144,19 +144,6 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32])
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-// Bytes (0, 1) or (2, 3) of a word of codes + 128, as two f16 (0x6400 | u is
-// 1024 + u).
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
-  const uint32_t u = __byte_perm(w, 0x64646464u, sel);
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 __device__ __forceinline__ void stmatrix_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b),
                "r"(c), "r"(d)
@@ -174,13 +161,13 @@ __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
 // The lowest n bits.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// N consecutive elements (8 or 16) of a result row.
-template <typename T, int N>
-__device__ __forceinline__ void store_row(T *dst, const float (&v)[N], int vec) {
+// 8 consecutive elements of a result row.
+template <typename T>
+__device__ __forceinline__ void store_row(T *dst, const float (&v)[8], int vec) {
   if (vec) {
     constexpr int W = 16 / sizeof(T);
 #pragma unroll
-    for (int e = 0; e < N; e += W) {
+    for (int e = 0; e < 8; e += W) {
       uint4 w;
       T *x = reinterpret_cast<T *>(&w);
 #pragma unroll
@@ -189,7 +176,7 @@ __device__ __forceinline__ void store_row(T *dst, const float (&v)[N], int vec) 
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < N; e++) dst[e] = from_f32<T>(v[e]);
+    for (int e = 0; e < 8; e++) dst[e] = from_f32<T>(v[e]);
   }
 }
 
@@ -240,16 +227,16 @@ __device__ __forceinline__ void load_queries(const T *src, bool vec, float scale
     if constexpr (sizeof(T) == 2) {  // 8 elements: a chunk's row
       uint32_t h[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) h[e] = pack_h2(to_f32<T>(x[2 * e]) * up, to_f32<T>(x[2 * e + 1]) * up);
+      for (int e = 0; e < 4; e++) h[e] = pack_f16(to_f32<T>(x[2 * e]) * up, to_f32<T>(x[2 * e + 1]) * up);
       *(uint4 *)(hi + (i * 4 + piece) * 2048) = make_uint4(h[0], h[1], h[2], h[3]);
     } else {  // 4 elements: half of it
       uint32_t h[2], l[2];
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const float a = to_f32<T>(x[2 * e]) * up, b = to_f32<T>(x[2 * e + 1]) * up;
-        h[e] = pack_h2(a, b);
+        h[e] = pack_f16(a, b);
         const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&h[e]));
-        l[e] = pack_h2(a - y.x, b - y.y);
+        l[e] = pack_f16(a - y.x, b - y.y);
       }
       const int at = (i * 2 + (piece >> 1)) * 2048 + (piece & 1) * 8;
       *(uint2 *)(hi + at) = make_uint2(h[0], h[1]);
@@ -451,10 +438,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               const uint64_t b = pack2(exp2_approx(lo_of(a)), exp2_approx(hi_of(a)));
               l2 = fadd2(l2, b);
               const uint64_t v = fmul2(b, pack2(wf[h], wf[h]));
-              w[e] = pack_h2(lo_of(v), hi_of(v));
+              w[e] = pack_f16(lo_of(v), hi_of(v));
               if (SPLIT) {
                 const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
-                w[16 + e] = pack_h2(lo_of(v) - y.x, hi_of(v) - y.y);
+                w[16 + e] = pack_f16(lo_of(v) - y.x, hi_of(v) - y.y);
               }
             }
             if constexpr (SPLIT) {
@@ -607,7 +594,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = acc[e] * inv * unit;
-            store_row<T, 8>(dst, acc, vec_o);
+            store_row<T>(dst, acc, vec_o);
             if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
           }
@@ -704,8 +691,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const uint32_t y = a[e] ^ 0x80808080u;
-              o[2 * e] = codes_f16(y, 0x4140);
-              o[2 * e + 1] = codes_f16(y, 0x4342);
+              o[2 * e] = two_f16(y, kLow);
+              o[2 * e + 1] = two_f16(y, kHigh);
             }
             const int tok = w * 32 + i * 8 + (lane & 7), kc = h * 8 + (lane >> 3) * 2;
             *(uint4 *)(kd + (kc * 128 + tok) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -741,8 +728,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const uint32_t y = a[e] ^ 0x80808080u;
-              o[2 * e] = codes_f16(y, 0x4140);
-              o[2 * e + 1] = codes_f16(y, 0x4342);
+              o[2 * e] = two_f16(y, kLow);
+              o[2 * e + 1] = two_f16(y, kHigh);
             }
             // matrices p = 0..3 then 4..7; lane gives the address of row (lane & 7) of matrix lane / 8
             const uint32_t at = vd + (uint32_t)(((w * 4 + i) * D + h * 64 + (lane >> 3) * 8 + (lane & 7)) * 16);

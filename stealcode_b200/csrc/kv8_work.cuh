@@ -197,6 +197,20 @@ __device__ __forceinline__ bool next_piece(const AttendArgs &p, const WorkGrid &
 // Workspace slot of part k of the item that starts in block c0.
 __device__ __forceinline__ int part_slot(int c0, int k) { return k == 0 ? 2 * c0 + 1 : 2 * (c0 + k); }
 
+// Bytes (0, 1) or (2, 3) of a word of codes, each with its top bit flipped
+// (code + 128), as two f16: 0x6400 | u is 1024 + u.
+__device__ __forceinline__ uint32_t two_f16(uint32_t w, uint32_t sel) {
+  const uint32_t u = __byte_perm(w, 0x64646464u, sel);
+  const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+constexpr uint32_t kLow = 0x4140, kHigh = 0x4342;
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -54,7 +54,6 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-
 class _Cache(ctypes.Structure):
     _fields_ = [(x, c_void_p) for x in ("k", "v", "k_scale", "v_scale", "table", "length", "refs", "status")] + \
                [(x, c_int64) for x in ("n_layers", "n_pages", "n_seqs", "max_pages")] + \
@@ -231,7 +230,8 @@ class KvCache8:
         A query at position p sees the tokens t <= p that still have a page and, with a window,
         t > p - window or t < sinks.  Returns out (q's type and shape), and with ``return_lse`` also the
         log-sum-exp of the scores, f32 [rows, n_heads].  A query that sees nothing: 0, -inf.
-        ``max_len``: no sequence is longer (sizes the launch).  ``scale``: head_dim ** -0.5 if None."""
+        ``max_len``: no sequence is longer (sizes the launch).  ``scale``: head_dim ** -0.5 if None.
+        An 8-bit cache serves and is not trained through: the result carries no gradient, whatever q does."""
         if q.dim() != 3 or q.shape[1] < 1:
             raise ValueError("q has to be [rows, n_heads, head_dim]")
         rows, heads = q.shape[:2]
@@ -320,4 +320,4 @@ class KvCache8:
         self.status.zero_()
 
 
-__all__ = ["KvCache8", "_lib"]
+__all__ = ["KvCache8"]
