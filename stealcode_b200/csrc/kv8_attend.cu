@@ -27,14 +27,16 @@
 // to a tile, so few rows waste little): both products contract over an axis
 // whose order is free, so K's and V's lanes take the 16 consecutive bytes
 // that they load, and nothing passes through shared memory.  The next step's
-// codes are sent to L2 meanwhile (64 streams: 143 us without).
+// codes are sent to L2 meanwhile (64 streams: a seventh more without).
 //
-// Measured: 64 sequences of 512-16384 tokens, 32 query heads on 8, bf16: 126
-// us, 4.8 TB/s of codes (of 6.5 measured for a copy); 4 of 65-131 k tokens: 144
-// us, 5.5 TB/s.  What is left is instructions: about 480 a warp and 16 tokens,
-// of them 160 to turn codes into f16, at half of the issue slots.  Short pasts
-// are latency (entry, page, codes, join: 2-3 us an item): 256 x 7 rows over a
-// window of 560, f32, take 86 us for 210 MB.
+// Measured as whole calls, one after the other (GPUs of one kind differ: the
+// first case takes 130 to 139 us): 64 sequences of 512-16384 tokens, 32 query
+// heads on 8, bf16: 138 us, 4.4 TB/s of codes (of 6.5 measured for a copy); 4
+// of 65-131 k tokens: 167 us, 4.7 TB/s.  What is left is instructions: about
+// 495 a warp and 16 tokens, of them 160 to turn codes into f16, at 59 % of the
+// issue slots; the ALU pipe is at 51 %.  Short pasts are latency (entry, page,
+// codes, join: 2-3 us an item): 256 x 7 rows over a window of 560, f32, take
+// 88 us for 210 MB.
 #include <atomic>
 
 #include "kv8_work.cuh"

@@ -31,10 +31,10 @@
 // lane's 16 loaded bytes give stmatrix without a shuffle; the epilogue undoes
 // it.  f32 queries and weights are hi + lo pairs of f16: twice the products.
 //
-// Measured: a prompt of 4096 tokens, 32 heads of 128 on 8, bf16: 254 us, 542
+// Measured: a prompt of 4096 tokens, 32 heads of 128 on 8, bf16: 253 us, 544
 // TFLOP/s of the visible pairs (of 1642 measured for bf16 products); 64 x 750
-// f32 frames, 8 heads: 386 us; four chunks of 301-1024 tokens, 16 heads of 64
-// on 4, window 2048: 87 us.  Bound by a row tile's chain: softmax 3 k cycles,
+// f32 frames, 8 heads: 382 us; four chunks of 301-1024 tokens, 16 heads of 64
+// on 4, window 2048: 88 us.  Bound by a row tile's chain: softmax 3 k cycles,
 // its two products 1.6 k (M 128 from shared memory takes 102 cycles a 16-deep
 // step instead of 64), a barrier wake-up after each; the tensor pipe is a
 // quarter busy.  Items of few key tiles also pay for queries, result and, where
