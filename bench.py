@@ -57,8 +57,9 @@ Multi-GPU: one process per GPU (torchrun); every rank encodes its own 256
 streams with its own weight copy (streams are independent: no collective on
 the data path; weak scaling).
 
-`--impl reference` times the reference's CPU path (the oracle port above,
-all host threads) on a bounded sample per step, rank 0 only.
+`--impl reference` prints that the reference is unavailable, and why: it
+cannot be built here, and this repository's port of its CPU path is no
+reference arm (`cpu_baseline` above times that).
 """
 from __future__ import annotations
 
@@ -268,42 +269,8 @@ def cpu_gemm_sample(budget_s=2.0):
 def run_reference(args, rank):
     if rank != 0:
         return
-    import oracle
-
-    m = encoder_model()
-    n_streams = 2
-    # one reference step = one 560 ms chunk for 2 streams (the GPU arm's step
-    # for 256 streams, sampled); state carries across steps like a stream
-    encs = [oracle.StreamingEncoder(m) for _ in range(n_streams)]
-    from stealcode_b200 import model
-
-    total = args.warmup + args.steps
-    mel = model.mel_stream(MODEL_SEED + 1, n_streams, MEL_PER_STEP * total, m.config.feat_in)
-    times = []
-    for i in range(total):
-        a, b = MEL_PER_STEP * i, MEL_PER_STEP * (i + 1)
-        if i == args.warmup:
-            before = phase_sum(encs)
-        t0 = time.perf_counter()
-        for z in range(n_streams):
-            assert encs[z].encode_new(mel[z, :b], a, b) == 0
-        if i >= args.warmup:
-            times.append(time.perf_counter() - t0)
-    after = phase_sum(encs)
-    phases = {k: after[k] - before[k] for k in after}
-    value = n_streams * AUDIO_S_PER_STEP * len(times) / sum(times)
-    cores = oracle.num_cpus()
-    sample = (f"{n_streams} streams x 1 chunk per step (steps {args.warmup}..{total - 1} of the streams), "
-              "oracle StreamingEncoder per stream with the reference's threading, AVX2 lanes and GEMM dispatch")
-    line = {"impl": "reference", "metric": METRIC, "value": value, "unit": UNIT, "n_gpus": args.gpus,
-            "steps": args.steps, "warmup": args.warmup, "ms_per_step": 1e3 * sum(times) / len(times),
-            "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "int8+f32",
-            "data": "synthetic", "config": {"workload": WORKLOAD, "streams_per_step": n_streams,
-                                            "chunk_ms": 560, "layers": N_LAYERS},
-            "cpu_baseline": {"value": value, "unit": UNIT, "cores": cores, "kind": "port", "sample": sample,
-                             "phases_s": phases},
-            "e2e": {"value": value, "unit": UNIT, "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}}
-    print(json.dumps(line), flush=True)
+    print(json.dumps({"impl": "reference", "unavailable": "the reference is a Rust (nightly) Cargo workspace without "
+                      "Python packaging; there is no Rust toolchain here to build it"}), flush=True)
 
 
 # ------------------------------------------------------------ GPU path ---
