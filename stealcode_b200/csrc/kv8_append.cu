@@ -130,9 +130,12 @@ __global__ void __launch_bounds__(128) append_block_kernel(const AppendArgs p, i
         found[0] = i;
         found[1] = slot - a;
       }
+    }
+    if (blockIdx.x == 0) {  // one block sees every entry, also those that take no slot
       int64_t row0;
-      int count;  // block 0 sees every entry, also those that take no slot
-      if (blockIdx.x == 0 && !p.b.rows(i, row0, count)) atomicOr(p.c.status, kBadRows);
+      int count;
+      for (int i = tid; i < p.b.m; i += 128)
+        if (!p.b.rows(i, row0, count)) atomicOr(p.c.status, kBadRows);
     }
     __syncthreads();
     entry = found[0];
@@ -302,14 +305,15 @@ __global__ void __launch_bounds__(128) rows_kernel(const RowsArgs p) {
   if (unit >= p.b.total) return;
   int i = -1;
   if (p.b.cu) {
-    for (int e = lane; e < p.b.m; e += 32) {
+    for (int e = lane; e < p.b.m; e += 32)
+      if (unit >= p.b.cu[e] && unit < p.b.cu[e + 1]) i = e;
+    i = __reduce_max_sync(0xffffffffu, i);
+    if (unit == 0) {  // one warp sees every entry, also those that hold no row
       int64_t start;
       int count;
-      const bool ok = p.b.rows(e, start, count);
-      if (unit >= start && unit < start + count) i = e;
-      if (unit == 0 && !ok) atomicOr(c.status, kBadRows);
+      for (int e = lane; e < p.b.m; e += 32)
+        if (!p.b.rows(e, start, count)) atomicOr(c.status, kBadRows);
     }
-    i = __reduce_max_sync(0xffffffffu, i);
   } else {
     i = (int)((uint32_t)unit / (uint32_t)p.b.n);
   }
