@@ -50,6 +50,11 @@ namespace kv8 {
 
 constexpr int kTileRows = 256, kTileKeys = 128;
 constexpr int kTileThreads = 768;  // 23 warps work; setmaxnreg takes whole warpgroups
+// Registers a thread: 80 at launch, which the 16 softmax warps keep; the four
+// product warps give 32 each to the converters (16 * 80 + 4 * 112 + 4 * 48 = 24 * 80).
+// With 72 for the softmax and 128 for the converters the softmax spills into
+// its loop: a prompt of 4096 tokens 274 us, so 247.
+constexpr int kTileRegs = 80;
 // An item's queries and result cost about as much as three tiles (a prompt of
 // 4096 tokens with 2, 3, 5, 8: 271, 254, 259, 273 us).
 constexpr int kTileOver = 3;
@@ -68,6 +73,7 @@ constexpr float kGain = 256.0f, kGainLog2 = 8.0f, kBigGain = 0x1p-40f, kBigScale
 constexpr float kToBig = 0x1p-48f, kFromBig = 0x1p48f, kToBigLog2 = -48.0f;
 constexpr float kLeastLog2 = -100.0f;  // of vs * gain
 constexpr float kBigSum = 0x1p60f;     // sums above it are not scaled by 2^48
+constexpr float kPartUnit = 0x1p-8f;   // of a part's output: results from 1e-30 to f32's largest have room
 
 // l * 2^d for a sum l, f = 2^d: with scales far apart 2^d can underflow
 // where the product does not.
@@ -290,7 +296,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   if (warp < 16) {
     // ================= softmax =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int q = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const int pair = 2 + q * 4 + (warp & 3);  // named barrier of this warp and the one with the rows' other half
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -474,8 +479,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           tc_fence_after();
         }
         const int pr = q * 128 + row;  // row of the item
-        const float inv = pc.whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        const float unit = pc.whole ? 1.0f / (kTileShift * (big ? kBigGain : kGain)) : 1.0f;
+        // A whole item: O / (l * units).  A part: its sum is brought to [1, 2), its
+        // output along with it and, whatever the gain was, to units of kPartUnit:
+        // parts join under one reference, and nothing leaves f32's range.
+        const float units = kTileShift * (big ? kBigGain : kGain);
+        float inv = l == 0.0f ? 0.0f : 1.0f / l, unit = 1.0f / units;
+        if (!pc.whole && l > 0.0f && l < INFINITY) {
+          const uint32_t bits = __float_as_uint(l);
+          const int k = (int)(bits >> 23) - 127;
+          inv = exp2_approx((float)-k);
+          unit *= kPartUnit;
+          m += (float)k;
+          l = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
+        }
         T *dst = (T *)p.out + (en.row0 + j) * p.o_row + hq * p.o_head;
         // A whole item's rows go through the queries' shared memory (their
         // last product has completed), 16-byte pieces swizzled by the row, so
@@ -543,7 +559,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (p.lse) p.lse[(en.row0 + j) * p.n_heads + hq] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
           } else {
             part[kTileRows * D + pr] = m;
-            part[kTileRows * D + kTileRows + pr] = big ? -l : l;  // the sign tells of the gain
+            part[kTileRows * D + kTileRows + pr] = l;
           }
         }
         tc_fence_before();  // O has been read before the next piece's first product overwrites it
@@ -565,7 +581,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int u = tid; u < nr * (D / 8); u += 512) {
             const int rr = u / (D / 8), d0 = u % (D / 8) * 8;
             float top = -INFINITY, sum = 0.0f, acc[8];
-            bool any_big = false;
 #pragma unroll
             for (int e = 0; e < 8; e++) acc[e] = 0.0f;
 #pragma unroll 4
@@ -576,24 +591,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               const float now = fmaxf(top, pm);
               const float old = now == -INFINITY ? 1.0f : exp2_approx(top - now);
               const float f = pm == -INFINITY ? (pl != pl ? pl : 0.0f) : exp2_approx(pm - now);
-              sum = (now == -INFINITY ? sum : scale_sum(sum, top - now, old)) +
-                    (pm == -INFINITY ? f : scale_sum(fabsf(pl), pm - now, f));
               top = now;
-              const bool was = any_big;
-              any_big |= signbit(pl);
-              const float fo = any_big != was ? old * kToBig : old, fv = any_big && !signbit(pl) ? f * kToBig : f;
+              sum = sum * old + f * pl;
               const float v[8] = {va.x, va.y, va.z, va.w, vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-              for (int e = 0; e < 8; e++) acc[e] = acc[e] * fo + fv * v[e];
+              for (int e = 0; e < 8; e++) acc[e] = acc[e] * old + f * v[e];
             }
             int j2, h2;
             en.row(g, rr, j2, h2);
             h2 += pc.head * g.group;
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const float unit = 1.0f / (kTileShift * (any_big ? kBigGain : kGain));
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * kPartUnit);
             T *dst = (T *)p.out + (en.row0 + j2) * p.o_row + h2 * p.o_head + d0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) acc[e] = acc[e] * inv * unit;
+            for (int e = 0; e < 8; e++) acc[e] *= inv;
             store_row<T>(dst, acc, vec_o);
             if (p.lse && d0 == 0)
               p.lse[(en.row0 + j2) * p.n_heads + h2] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp < 20) {
     // ================= converters =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     const int w = warp - 16;
     constexpr int HF = D / 64;
     const int nblk = c.page / c.block;
@@ -886,6 +896,17 @@ static int launch_tile(const AttendArgs &a, int sm_count, cudaStream_t st) {
   const size_t bytes = C::kOperands + sizeof(TileShared);
   const int rc = raise_smem_limit((const void *)attend_tile_kernel<D, T>, bytes, limit);
   if (rc) return rc;
+  // the converters would wait for registers that a smaller launch does not have
+  static std::atomic<bool> checked{false};
+  if (!checked.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes f;
+    SC_CUDA(cudaFuncGetAttributes(&f, (const void *)attend_tile_kernel<D, T>));
+    if (f.numRegs < kTileRegs) {
+      set_error("kv8_attend: built with %d registers a thread, %d are needed", f.numRegs, kTileRegs);
+      return kErrUnsupported;
+    }
+    checked.store(true, std::memory_order_relaxed);
+  }
   attend_tile_kernel<D, T><<<sm_count, kTileThreads, bytes, st>>>(a, g, vq, vo);
   SC_CUDA(cudaGetLastError());
   note_launch();
