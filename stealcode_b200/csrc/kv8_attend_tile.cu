@@ -31,10 +31,10 @@
 // lane's 16 loaded bytes give stmatrix without a shuffle; the epilogue undoes
 // it.  f32 queries and weights are hi + lo pairs of f16: twice the products.
 //
-// Measured: a prompt of 4096 tokens, 32 heads of 128 on 8, bf16: 253 us, 544
+// Measured: a prompt of 4096 tokens, 32 heads of 128 on 8, bf16: 247 us, 557
 // TFLOP/s of the visible pairs (of 1642 measured for bf16 products); 64 x 750
-// f32 frames, 8 heads: 382 us; four chunks of 301-1024 tokens, 16 heads of 64
-// on 4, window 2048: 88 us.  Bound by a row tile's chain: softmax 3 k cycles,
+// f32 frames, 8 heads: 385 us; four chunks of 301-1024 tokens, 16 heads of 64
+// on 4, window 2048: 86 us.  Bound by a row tile's chain: softmax 3 k cycles,
 // its two products 1.6 k (M 128 from shared memory takes 102 cycles a 16-deep
 // step instead of 64), a barrier wake-up after each; the tensor pipe is a
 // quarter busy.  Items of few key tiles also pay for queries, result and, where
@@ -56,7 +56,7 @@ constexpr int kTileThreads = 768;  // 23 warps work; setmaxnreg takes whole warp
 // its loop: a prompt of 4096 tokens 274 us, so 247.
 constexpr int kTileRegs = 80;
 // An item's queries and result cost about as much as three tiles (a prompt of
-// 4096 tokens with 2, 3, 5, 8: 271, 254, 259, 273 us).
+// 4096 tokens with 2, 3, 5, 8, an earlier version: 271, 254, 259, 273 us).
 constexpr int kTileOver = 3;
 constexpr float kTileShift = 256.0f, kTileSlack = 7.0f;
 constexpr float kTinyFactor = 1e-37f;  // a score factor of 0 would make NaN of a hidden score's -inf
